@@ -129,7 +129,7 @@ def _plain_loss(state):
         z = z + state["bias"]
     top = z.amax(1, keepdim=True)
     lse = top[:, 0] + torch.log(torch.exp(z - top).sum(1))
-    there = targets >= 0
+    there = targets >= 0                # padding is left out: its loss and its log-sum are 0
     at = targets.clamp(min=0)[:, None]
     loss = torch.where(there, lse - z.gather(1, at)[:, 0], torch.zeros_like(lse))
     return z, lse, loss, there, at
@@ -160,8 +160,8 @@ def run(state):
         sums.index_add_(0, torch.where(ids >= 0, ids, torch.full_like(ids, state["rows"])), state["grad"].float())
         return (sums[:-1] * state["scale"]).to(state["grad"].dtype)
     if op == "loss":
-        _, lse, loss, _, _ = _plain_loss(state)
-        return loss, lse
+        _, lse, loss, there, _ = _plain_loss(state)
+        return loss, lse * there
     if op == "train":
         z, lse, loss, there, at = _plain_loss(state)
         weights = there * state["weights"]
@@ -171,7 +171,7 @@ def run(state):
         dx = torch.matmul(g, state["table"].float()) * state["scale"]
         dtable = torch.matmul(g.t(), state["x"].float()) * state["scale"]
         dbias = None if state["bias"] is None else g.sum(0)
-        return loss, lse, dx.to(state["x"].dtype), dtable.to(state["table"].dtype), dbias
+        return loss, lse * there, dx.to(state["x"].dtype), dtable.to(state["table"].dtype), dbias
     norm = torch.stack([(g.float() * g.float()).sum() for g in state["grads"]]).sum().sqrt()
     factor = torch.clamp(state["most"] / norm, max=1.0)
     return [norm] + [(g.float() * factor).to(g.dtype) for g in state["grads"]]
@@ -222,8 +222,8 @@ def exact(case, seed):
         z = given["scale"] * (x[a:a + many] @ w.T)
         if given["bias"] is not None:
             z += given["bias"].double()
-        lse[a:a + many] = torch.logsumexp(z, 1)
         live = torch.nonzero(t[a:a + many] >= 0)[:, 0]
+        lse[a + live] = torch.logsumexp(z, 1)[live]
         hit = t[a:a + many][live]
         loss[a + live] = lse[a + live] - z[live, hit]
         if op == "train":
