@@ -279,6 +279,65 @@ int mfsgd_hip_als_step_f64(double *latent, const double *fixed, const int64_t *r
                            const double *vals, int64_t n_rows, int64_t n_cols, int64_t nnz, int32_t k, double lambda,
                            void *stream);
 
+/* ---- minibatch operators on factor tables: lookup of a batch of rows and its gradient, the softmax (ranking) loss over
+ * the whole catalogue and its gradient, the global norm of a set of gradients and their clipping.  No counterpart in the
+ * reference (it updates rating by rating); they stand beside mfsgd_hip_implicit_z_* (rows gathered and scaled) and
+ * mfsgd_hip_topn_f32 (the same product of user rows and item rows).
+ *  - dtype: MFSGD_F32 or MFSGD_BF16, the type of every table, batch and gradient of a call; sums, statistics, biases,
+ *    weights, losses and norms are float32 or wider;
+ *  - *_stride: distance between rows in elements (>= d), so that zero-padded device rows can be used as they are;
+ *  - ids and targets are int32.  A negative one is padding: a zero row, no gradient, a loss of 0.  One past the table's end
+ *    is never followed: its row (its loss) comes out as NaN and it adds no gradient;
+ *  - workspace: device memory, 16-byte aligned, of at least the bytes the matching *_workspace call names (host-only, -1 on
+ *    bad arguments).  Nothing in it is kept from call to call; calls that can overlap need one each (two streams, two
+ *    captured graphs);
+ *  - no call allocates, synchronises or clears memory with a memset: all of them can be captured into a graph;
+ *  - fixed summation orders, no floating-point atomics: a call repeated on the same inputs gives the same bits;
+ *  - all device pointers must belong to the current device and to `stream`'s. */
+#define MFSGD_F32 0
+#define MFSGD_BF16 1
+
+/* out[t] = scale * table[ids[t]], t < n; out is [n][d] without gaps.  Any d >= 1. */
+int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows, int32_t d, const int32_t *ids, int64_t n,
+                        float scale, int32_t dtype, void *out, void *stream);
+/* out[v] = scale * sum of grad[t] over the t with ids[t] == v, in the order of t; a row no id names is set to zero.
+ * accumulate != 0: the sum is added to out[v] (rounded once), rows no id names stay as they are.  n < 2^31 - 1. */
+int64_t mfsgd_embedding_grad_workspace(int64_t n, int64_t n_rows, int32_t d);
+int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_t *ids, int64_t n, int64_t n_rows, int32_t d,
+                             float scale, int32_t dtype, int32_t accumulate, void *out, int64_t out_stride,
+                             void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of x [n][d] against the items' table [n_items][d], 1 <= d <= 256, without keeping the n x n_items
+ * logits z_rv = scale * x_r . table_v + bias_v (bias may be NULL):
+ *   lse[r] = log sum_v exp z_rv,   loss[r] = lse[r] - z_{r, targets[r]}.
+ * A bias of -inf (or below -2e38) takes an item out of the catalogue; a row whose target is out has the loss +inf, with
+ * every item out also the lse -inf and no gradient.  A padding row's x is not looked at: loss and lse are 0.
+ * scale > 0. */
+int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads);
+int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets,
+                           const float *bias, int64_t n, int64_t n_items, int32_t d, float scale, int32_t dtype,
+                           float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+/* The same with the gradients of sum_r weight * weights[r] * loss[r] (weights may be NULL: all 1):
+ *   G_rv = weight * weights[r] * (exp(z_rv - lse[r]) - [v == targets[r]]),
+ *   dx = scale * G . table  [n][d],   dtable = scale * G^T . x  [n_items][d],   dbias[v] = sum_r G_rv (NULL: not wanted).
+ * dx and dtable are without gaps, of `dtype`, rounded once from fp32 sums. */
+int mfsgd_hip_softmax_loss_grads(const void *x, int64_t x_stride, const void *table, int64_t table_stride,
+                                 const int32_t *targets, const float *bias, const float *weights, float weight, int64_t n,
+                                 int64_t n_items, int32_t d, float scale, int32_t dtype, float *loss, float *lse, void *dx,
+                                 void *dtable, float *dbias, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* norm[0] = sqrt(sum over all tensors of the sum of squares), summed in float64.  h_grads / h_sizes / h_dtypes are HOST
+ * arrays of n_tensors device pointers, element counts (0 allowed) and types; they are read before the call returns. */
+int64_t mfsgd_grad_norm_workspace(const int64_t *h_sizes, int32_t n_tensors);
+int mfsgd_hip_grad_norm(const void *const *h_grads, const int64_t *h_sizes, const int32_t *h_dtypes, int32_t n_tensors,
+                        float *norm, void *workspace, int64_t workspace_bytes, void *stream);
+/* h_out[i] = h_grads[i] * min(1, max_norm / norm); h_out NULL, or h_out[i] == h_grads[i]: in place, and then nothing is
+ * written where norm <= max_norm.  max_norm > 0.  A norm that is not a number makes every gradient not a number, an
+ * infinite one makes the finite gradients zero. */
+int mfsgd_hip_clip_grads(const void *const *h_grads, void *const *h_out, const int64_t *h_sizes, const int32_t *h_dtypes,
+                         int32_t n_tensors, float max_norm, float *norm, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+
 /* ---- multi-GPU DSGD ring, host side (SURVEY.md 8(b) `mfsgd_dsgd_*`, 8(e)).  No counterpart in the reference (it has no
  * multi-device path); the rule is its FPSGD invariant (RayBlockScheduler.py:50-62) one level up: users are cut into
  * `world` contiguous super-stripes and items into `world` contiguous shards, both on boundaries of the ubp x ibp block

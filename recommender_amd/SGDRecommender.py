@@ -27,6 +27,7 @@ import numpy as np
 
 from . import _abi
 from .numba_methods import mse, mse2, rmse_exact, sgd, sgd2  # noqa: F401  (re-exported like `from numba_methods import *`)
+from .minibatch import clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
 from .Recommender import Recommender
 from .SubSample import SubSample
 
@@ -634,6 +635,23 @@ class ExplicitMF(Recommender):
                                                  _abi.stream_ptr()))
         torch.cuda.synchronize()
         return items[:, :n].cpu().numpy(), scores[:, :n].cpu().numpy()
+
+    @staticmethod
+    def ranking_step(users, items, user_vecs, item_vecs, b_i=None, lr=0.1, max_norm=None, scale=1.0):
+        """One minibatch step of the ranking objective that `top_n` answers for: lowers the mean over the batch of
+        -log softmax(scale * user_vecs[users] @ item_vecs.T + b_i)[items], in place on the given ROCm tensors (float32 or
+        bfloat16 factors, float32 b_i; users and items int32, an item < 0 is padding).  With `max_norm` the gradients of
+        all factors are clipped to it first.  Returns (loss [n], norm of the gradients); asynchronous, no host copies."""
+        n = int(users.shape[0])
+        x = embedding(user_vecs, users)
+        loss, _, dx, dq, db = softmax_loss_grads(x, item_vecs, items, bias=b_i, scale=scale, weights=1.0 / max(n, 1))
+        dp = embedding_grad(dx, users, user_vecs.shape[0])
+        pairs = [(user_vecs, dp), (item_vecs, dq)] + ([(b_i, db)] if b_i is not None else [])
+        grads = [g for _, g in pairs]
+        norm = grad_norm(grads) if max_norm is None else clip_grads(grads, max_norm)
+        for t, g in pairs:
+            t.sub_(g, alpha=lr)
+        return loss, norm
 
     def recommend(self, users, n=10):
         """Top-n items (current id space) for `users` under the trained model's predictor without the implicit term."""

@@ -8,6 +8,8 @@ from .RayBlockScheduler import BlockScheduler, consumer  # noqa: F401
 from .SGDRecommender import ExplicitMF  # noqa: F401
 from .Recommender import Recommender  # noqa: F401
 from .numba_methods import sgd, sgd2, block_sgd, mse, mse2, rmse_exact  # noqa: F401
+from .minibatch import (embedding, embedding_grad, softmax_loss, softmax_loss_grads, grad_norm, clip_grads)  # noqa: F401
 
 __all__ = ["ExplicitMF", "Recommender", "BlockScheduler", "SubSample", "consumer",
-           "sgd", "sgd2", "block_sgd", "mse", "mse2", "rmse_exact"]
+           "sgd", "sgd2", "block_sgd", "mse", "mse2", "rmse_exact",
+           "embedding", "embedding_grad", "softmax_loss", "softmax_loss_grads", "grad_norm", "clip_grads"]

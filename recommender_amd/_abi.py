@@ -83,6 +83,18 @@ SIGNATURES = {
     "mfsgd_grid_col_times": (C.c_int, [c_vp, c_vp, c_vp]),
     "mfsgd_hip_epoch_f32": (C.c_int, _sig_epoch(c_f32)),
     "mfsgd_hip_epoch_f64": (C.c_int, _sig_epoch(c_f64)),
+    "mfsgd_hip_embedding": (C.c_int, [c_vp, c_i64, c_i64, c_i32, c_vp, c_i64, c_f32, c_i32, c_vp, c_vp]),
+    "mfsgd_embedding_grad_workspace": (c_i64, [c_i64, c_i64, c_i32]),
+    "mfsgd_hip_embedding_grad": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_f32, c_i32, c_i32, c_vp, c_i64, c_vp,
+                                           c_i64, c_vp]),
+    "mfsgd_softmax_loss_workspace": (c_i64, [c_i64, c_i64, c_i32, c_i32, c_i32]),
+    "mfsgd_hip_softmax_loss": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_f32, c_i32, c_vp, c_vp,
+                                         c_vp, c_i64, c_vp]),
+    "mfsgd_hip_softmax_loss_grads": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_f32, c_i64, c_i64, c_i32, c_f32,
+                                               c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "mfsgd_grad_norm_workspace": (c_i64, [c_vp, c_i32]),
+    "mfsgd_hip_grad_norm": (C.c_int, [c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp]),
+    "mfsgd_hip_clip_grads": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_f32, c_vp, c_vp, c_i64, c_vp]),
 }
 
 

@@ -1,0 +1,608 @@
+// softmax_loss.hip - softmax cross entropy of a batch of rows against a whole catalogue of items, and its gradient, without
+// ever keeping the n x n_items logits (gfx950, MI355X).
+//
+//   z_rv = scale x_r.w_v + b_v,   lse_r = log sum_v exp z_rv,   loss_r = lse_r - z_{r,t_r}
+//   G_rv = g_r (exp(z_rv - lse_r) - [v = t_r]),   dX = scale G W,   dW = scale G^T X,   db = sum_r G_r
+//
+// One kernel shape does all the products (k_stream): a wave keeps 32 STATIONARY rows in registers and walks past tiles of
+// STREAMED rows in LDS.  With streamed rows as MFMA rows and stationary rows as MFMA columns a lane ends up with 16 logits
+// of ONE stationary row, so running maximum and sum are private to a lane, and the exponentials are, as they stand, the B
+// operand of the second product (the order of the streamed rows inside an operand is free, and the other operand, read
+// transposed from the same LDS tile, takes the same order).
+//   pass 1   stationary x, streamed items:  running maximum, sum and sum_v exp(z - m) w_v, in one walk over the items
+//   combine  joins the parts of the items' axis: lse, loss, dX
+//   pass 2   stationary items, streamed x:  the logits again, now with lse known:  dW, db
+// 8 n d V operations, two of the logits, against the 6 that cannot be avoided: keeping the logits would move 2 n V elements
+// to memory and back instead.
+//
+// The target's own term is left out of pass 1 and added in the combine, in fp32 from the rows themselves: 1 - p_t is then the
+// other items' share, not a difference of rounded numbers, and a well-learnt row's gradient (p_t near 1) keeps its digits.
+//
+// Types: bf16 rows are the operands as they are.  An fp32 row is split into three bf16 rows of 8 bits each (x = x0 + x1 + x2,
+// exact to 2^-24), and a product is the six products of order up to 2 - the three left out are below 2^-24 of it.  Six bf16
+// matrix instructions cost less than one fp32 instruction of the same shape (2.5 PFLOP/s against 157 TFLOP/s).  The
+// exponentials, too, are rounded to bf16 for the second product, as they are written to no memory (bf16 rows: one value of
+// 2^-9, the outputs' own rounding; fp32 rows: three).
+#include <algorithm>
+#include <math.h>
+#include "rows.h"
+
+namespace {
+
+#define LDS_AS __attribute__((address_space(3)))
+#define GLB_AS __attribute__((address_space(1)))
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// The running maximum follows a tile's only when it rose by more than this (log2): any reference will do as long as
+// nothing overflows, and a new one costs a multiplication of all sums.
+constexpr float SLACK = 8.f;
+
+enum { LOSS = 0, LOSS_SUMS = 1, TABLE = 2 };   // pass 1 without / with the weighted sums, pass 2
+
+struct StreamArgs {
+    const __bf16 *st, *sm;              // planes of stationary / streamed rows, DP wide, zero padded
+    int64_t st_stride, st_plane, sm_stride, sm_plane;
+    int64_t n_st, n_sm;
+    const int32_t *targets;             // of the x rows (padding and ids outside the table: -1)
+    const float *bias;                  // of the items, may be NULL
+    float c, inv_scale;                 // scale log2(e), 1 / scale
+    int32_t splits, row_tiles;
+    float *part_m, *part_s;             // pass 1 [splits][n_st]; pass 2: part_s = sums of G for the bias
+    float *part_o;                      // [splits][n_st][DP]
+    const float *row_init, *row_q, *row_g;   // pass 2: -lse / scale, g (1 - p_t), g (g: the row's weight, NULL: all 1)
+};
+
+template <int DP, int PL> struct Shape {
+    static constexpr int TB = (PL == 3 && DP > 32) ? 32 : 64;        // streamed rows a tile
+    static constexpr int CH = DP / 8;                                // 16-byte pieces of a row
+    static constexpr int BUF = PL * TB * DP * 2;                     // bytes of a tile
+    static constexpr int LDS = 2 * BUF + 2 * TB * 12;
+};
+
+// piece c of row r lies at piece c ^ swizzle(r): the 8 rows that a read touches at once then lie in different banks
+template <int CH> __device__ __forceinline__ int swizzle(int r) { return CH >= 8 ? (r & 7) : ((r >> 1) & 3); }
+
+template <int DP, int PL, int NW, int MODE>
+__global__ __launch_bounds__(NW * 64, (DP * PL > 256 ? 1 : 2)) void k_stream(const StreamArgs a)
+{
+    using S = Shape<DP, PL>;
+    constexpr int TB = S::TB, CH = S::CH, BUF = S::BUF, KS = DP / 16, DT = DP / 32;
+    constexpr int Q = BUF / (NW * 1024);
+    static_assert(BUF % (NW * 1024) == 0, "a tile is a whole number of 1 KB pieces per wave");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float *l_init = (float *)(lds + 2 * BUF);           // [2][TB]
+    float *l_g = l_init + 2 * TB;
+    int32_t *l_t = (int32_t *)(l_g + 2 * TB);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, kh = lane >> 5;
+
+    // consecutive workgroups go round the 8 XCDs: the row tiles that walk the same part of the streamed axis share one's L2
+    int split, rt;
+    if (a.splits % 8 == 0) {
+        const int j = blockIdx.x >> 3;
+        split = (j / a.row_tiles) * 8 + (blockIdx.x & 7);
+        rt = j % a.row_tiles;
+    } else {
+        split = blockIdx.x / a.row_tiles;
+        rt = blockIdx.x % a.row_tiles;
+    }
+    const int64_t st0 = ((int64_t)rt * NW + wave) * 32;
+    const int64_t st_row = std::min<int64_t>(st0 + col, a.n_st - 1);
+    const int64_t tiles = (a.n_sm + TB - 1) / TB;
+    const int64_t t0 = tiles * split / a.splits, t1 = tiles * (split + 1) / a.splits;
+
+    bf16x8 b[PL][KS];
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            b[p][s] = *(const bf16x8 *)(a.st + p * a.st_plane + st_row * a.st_stride + 16 * s + 8 * kh);
+
+    auto stage = [&](int64_t t, int buf) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int slot = (q * NW + wave) * 64 + lane;
+            const int p = slot / (TB * CH), r = slot / CH % TB, c = (slot % CH) ^ swizzle<CH>(slot / CH % TB);
+            const int64_t row = std::min<int64_t>(t * TB + r, a.n_sm - 1);
+            __builtin_amdgcn_global_load_lds((const GLB_AS void *)(a.sm + p * a.sm_plane + row * a.sm_stride + c * 8),
+                                             (LDS_AS void *)(lds + buf * BUF + (q * NW + wave) * 1024), 16, 0, 0);
+        }
+        if (tid < TB) {
+            const int64_t row = t * TB + tid;
+            const bool in = row < a.n_sm;
+            const int64_t rr = in ? row : a.n_sm - 1;
+            if constexpr (MODE == TABLE) {
+                l_init[buf * TB + tid] = in ? a.row_init[rr] : -INFINITY;
+                if (a.row_g) l_g[buf * TB + tid] = a.row_g[rr];
+                l_t[buf * TB + tid] = in ? a.targets[rr] : -1;
+            } else
+                l_init[buf * TB + tid] = in ? (a.bias ? a.bias[rr] * a.inv_scale : 0.f) : -INFINITY;
+        }
+    };
+
+    f32x16 o[MODE == LOSS ? 1 : DT];
+#pragma unroll
+    for (auto &v : o) v = (f32x16)(0.f);
+    float m = -INFINITY, sum = 0.f;
+    const int32_t target = MODE == TABLE ? -1 : a.targets[st_row];
+    const float b2 = (MODE == TABLE && a.bias) ? a.bias[st_row] * LOG2E : 0.f;
+
+    if (t0 < t1) stage(t0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int64_t t = t0; t < t1; ++t) {
+        const int buf = (int)((t - t0) & 1);
+        if (t + 1 < t1) stage(t + 1, buf ^ 1);
+        const char *tile = lds + buf * BUF;
+#pragma unroll 1
+        for (int sub = 0; sub < TB / 32; ++sub) {
+            // logits (in units of scale) of 32 streamed rows: acc[j] is row 8 (j / 4) + 4 kh + j % 4 for stationary row `col`
+            f32x16 acc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 v = *(const f32x4 *)(l_init + buf * TB + sub * 32 + 8 * j + 4 * kh);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[4 * j + i] = v[i];
+            }
+            const char *arow = tile + (sub * 32 + col) * DP * 2;
+            const int sw = swizzle<CH>(col);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                bf16x8 x[PL];
+#pragma unroll
+                for (int p = 0; p < PL; ++p) x[p] = *(const bf16x8 *)(arow + p * TB * DP * 2 + ((2 * s + kh) ^ sw) * 16);
+                if constexpr (PL == 3) {
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], b[0][s], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[2][s], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[1][s], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[0][s], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[1][s], acc, 0, 0, 0);
+                }
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[0][s], acc, 0, 0, 0);
+            }
+            float e[16];
+            if constexpr (MODE != TABLE) {
+                float top = acc[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) top = fmaxf(top, acc[j]);
+                const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.c;
+                const bool rise = top > m + SLACK;
+                if (__ballot(rise)) {
+                    const float f = rise ? __builtin_amdgcn_exp2f(m - top) : 1.f;    // the first tile: exp2(-inf) = 0
+                    if (rise) m = top;
+                    sum *= f;
+                    if constexpr (MODE == LOSS_SUMS) {
+#pragma unroll
+                        for (auto &v : o) v *= f;
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[j], a.c, -ref));
+                const uint32_t at = (uint32_t)(target - (int32_t)(t * TB + sub * 32));
+                if (__ballot(at < 32u)) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) e[j] = at == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
+                }
+                float s4[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);
+                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[j], a.c, b2));
+                if (a.row_g) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const f32x4 v = *(const f32x4 *)(l_g + buf * TB + sub * 32 + 8 * j + 4 * kh);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e[4 * j + i] *= v[i];
+                    }
+                }
+                // rows of the tile whose target is one of this wave's items: -g (1 - p_t) in the place of g p_t
+                const uint32_t at = (uint32_t)(l_t[buf * TB + sub * 32 + col] - (int32_t)st0);
+                uint32_t hits = (uint32_t)__ballot(at < 32u);
+                while (hits) {
+                    const int r = __builtin_ctz(hits);
+                    hits &= hits - 1;
+                    const int item = __builtin_amdgcn_readlane((int)at, r);
+                    const float g = -a.row_q[t * TB + sub * 32 + r];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) e[j] = (r == 8 * (j / 4) + 4 * kh + j % 4 && col == item) ? g : e[j];
+                }
+                if (a.part_s) {
+                    float s4[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);
+                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                }
+            }
+            if constexpr (MODE != LOSS) {
+                // o[dt][j] += sum over the 32 streamed rows of their column 32 dt + 8 (j / 4) + 4 kh + j % 4 times e
+                const int i = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    bf16x8 w[PL];
+                    {
+                        float rest[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) rest[q] = e[8 * k + q];
+#pragma unroll
+                        for (int p = 0; p < PL; ++p) {
+                            uint32_t u[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                u[q] = pack_bf16(rest[2 * q], rest[2 * q + 1]);
+                                if (p + 1 < PL) { rest[2 * q] -= bf16_lo(u[q]); rest[2 * q + 1] -= bf16_hi(u[q]); }
+                            }
+                            w[p] = __builtin_bit_cast(bf16x8, *(const uint4 *)u);
+                        }
+                    }
+                    const int r = sub * 32 + 16 * k + 4 * kh + (i >> 2);        // and r + 8: the same swizzle
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int piece = (4 * dt + 2 * g + ((i & 3) >> 1)) ^ swizzle<CH>(r);
+                        bf16x8 x[PL];
+#pragma unroll
+                        for (int p = 0; p < PL; ++p) {
+                            const char *src = tile + p * TB * DP * 2 + r * DP * 2 + piece * 16 + (i & 1) * 8;
+                            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)src);
+                            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(src + 8 * DP * 2));
+                            x[p] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+                        }
+                        if constexpr (PL == 3) {
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], w[0], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[2], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[1], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[0], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[1], o[dt], 0, 0, 0);
+                        }
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[0], o[dt], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+
+    if (st0 + col >= a.n_st) return;
+    const int64_t at = (int64_t)split * a.n_st + st0 + col;
+    if (MODE != TABLE || a.part_s) {
+        const float both = sum + __shfl_xor(sum, 32, 64);     // the two lanes of a row leave the kernel together
+        if (kh == 0) {
+            if constexpr (MODE != TABLE) a.part_m[at] = m;
+            a.part_s[at] = both;
+        }
+    }
+    if constexpr (MODE != LOSS) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = o[dt][4 * j + i];
+                *(f32x4 *)(a.part_o + at * DP + 32 * dt + 8 * j + 4 * kh) = v;
+            }
+    }
+}
+
+// rows -> planes of bf16, DP wide, columns from d on zero; with targets: the rows that take no part are zero, their target -1
+template <typename T, int PL>
+__global__ __launch_bounds__(256) void k_planes(const T *__restrict__ src, int64_t stride, int64_t n, int32_t d, int32_t dp,
+                                                const int32_t *__restrict__ targets, int64_t n_items, __bf16 *__restrict__ dst,
+                                                int32_t *__restrict__ targets_out)
+{
+    const int32_t per = dp / 8;
+    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p >= n * per) return;
+    const int64_t r = p / per;
+    const int32_t c = (int32_t)(p - r * per) * 8;
+    bool in = true;
+    if (targets) {
+        const int32_t t = targets[r];
+        in = (uint32_t)t < (uint64_t)n_items;
+        if (c == 0) targets_out[r] = in ? t : -1;
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = in && c + i < d ? load_f32(src + r * stride + c + i) : 0.f;
+#pragma unroll
+    for (int q = 0; q < PL; ++q) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            v[2 * i] -= bf16_lo(u[i]);
+            v[2 * i + 1] -= bf16_hi(u[i]);
+        }
+        *(uint4 *)(dst + (int64_t)q * n * dp + r * dp + c) = *(const uint4 *)u;
+    }
+}
+
+struct JoinArgs {
+    int64_t n, n_items, x_stride, w_stride;
+    int32_t d, dp, splits;
+    float scale, weight;
+    const int32_t *targets;
+    const float *bias, *weights, *part_m, *part_s, *part_o;
+    float *loss, *lse, *row_init, *row_q, *row_g;     // row_init NULL: no gradients
+};
+
+// One wave a row: joins the parts of the items' axis, adds the target's own term and writes loss, lse, the row's dX and what
+// pass 2 needs of the row.
+template <typename T>
+__global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__restrict__ x, const T *__restrict__ w, T *__restrict__ dx)
+{
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x;
+    const int32_t t = a.targets[r];
+    const bool in = (uint32_t)t < (uint64_t)a.n_items;
+    if (!in) {
+        if (lane == 0) {
+            a.loss[r] = a.lse[r] = t < 0 ? 0.f : NAN;
+            if (a.row_init) { a.row_init[r] = -INFINITY; a.row_q[r] = 0.f; if (a.row_g) a.row_g[r] = 0.f; }
+        }
+        if (dx) for (int c = lane; c < a.d; c += 64) store_f32(dx + r * a.d + c, 0.f);
+        return;
+    }
+    float dot = 0.f;
+    for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
+    const float z = (wave_sum(dot) * a.scale + (a.bias ? a.bias[t] : 0.f)) * LOG2E;      // the target's logit, log2
+    float m = -INFINITY;
+    bool bad = false;
+    for (int s = lane; s < a.splits; s += 64) {
+        m = fmaxf(m, a.part_m[(int64_t)s * a.n + r]);
+        bad |= !(a.part_s[(int64_t)s * a.n + r] >= 0.f);       // not a number
+    }
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+    const float top = fmaxf(m, z);
+    const bool none = top == -INFINITY && !(z != z) && !__ballot(bad);       // every item is out of the catalogue
+    // Everything relative to the target's logit unless it lies so far below that the others' share would overflow: the loss is
+    // then log1p(others), with no difference of nearly equal numbers in it
+    const bool near = z > m - 64.f;
+    const float ref = near ? z : (top == -INFINITY ? 0.f : top);
+    float sum = 0.f;
+    for (int s = lane; s < a.splits; s += 64) sum += a.part_s[(int64_t)s * a.n + r] * __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);
+    const float others = wave_sum(sum), own = __builtin_amdgcn_exp2f(z - ref), all = others + own;
+    const float log_all = near ? log1pf(others) : logf(all);
+    const float loss = none ? INFINITY : (near ? log_all : log_all + (ref - z) * LN2);
+    const float q = none ? 0.f : others / all;                 // 1 - p_t
+    if (lane == 0) {
+        a.loss[r] = loss;
+        a.lse[r] = none ? -INFINITY : log_all + ref * LN2;
+    }
+    if (!a.row_init) return;
+    const float g = a.weights ? a.weights[r] : 1.f;
+    if (lane == 0) {
+        a.row_init[r] = none ? -INFINITY : -((log_all + ref * LN2) / a.scale);
+        a.row_q[r] = q * g;
+        if (a.row_g) a.row_g[r] = none ? 0.f : g;
+    }
+    const float f = g * a.weight * a.scale;
+    for (int c = lane; c < a.d; c += 64) {
+        float v = 0.f;
+        for (int s = 0; s < a.splits; ++s)
+            v += a.part_o[((int64_t)s * a.n + r) * a.dp + c] * __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);
+        const float out = none ? 0.f : f * (v / all - q * load_f32(w + (int64_t)t * a.w_stride + c));
+        store_f32(dx + r * a.d + c, out);
+    }
+}
+
+// the parts of the rows' axis of pass 2, summed in order: dW and db
+template <typename T>
+__global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ part_o, const float *__restrict__ part_s, int32_t splits,
+                                                    int64_t n_items, int32_t d, int32_t dp, float f, float weight, T *__restrict__ dw,
+                                                    float *__restrict__ db)
+{
+    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p >= n_items * d) return;
+    const int64_t v = p / d;
+    const int32_t c = (int32_t)(p - v * d);
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += part_o[((int64_t)k * n_items + v) * dp + c];
+    store_f32(dw + p, s * f);
+    if (db && c == 0) {
+        float t = 0.f;
+        for (int k = 0; k < splits; ++k) t += part_s[(int64_t)k * n_items + v];
+        db[v] = t * weight;
+    }
+}
+
+struct LossPlan {
+    int dp, planes, nw1, splits1, rt1, splits2, rt2;
+    bool copy_w;
+    int64_t xp, wp, targets, m1, s1, o1, init, q, g, s2, o2, bytes;
+};
+
+int tile_rows(int dp, int planes) { return planes == 3 && dp > 32 ? 32 : 64; }
+
+// Parts an axis of `tiles` tiles is cut into so that `row_tiles` workgroups a part give the chip two per CU
+int parts_of(int64_t tiles, int64_t row_tiles, int64_t want)
+{
+    int64_t s = std::min(tiles, (want + row_tiles - 1) / row_tiles);
+    if (s > 8) s = s / 8 * 8;
+    return (int)std::max<int64_t>(1, s);
+}
+
+LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool grads)
+{
+    LossPlan p = {};
+    n = std::max<int64_t>(n, 1);
+    p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
+    p.planes = dtype == MFSGD_F32 ? 3 : 1;
+    const int tb = tile_rows(p.dp, p.planes);
+    p.nw1 = 4;
+    p.rt1 = (int)((n + 32 * p.nw1 - 1) / (32 * p.nw1));
+    p.splits1 = parts_of((n_items + tb - 1) / tb, p.rt1, 512);
+    p.rt2 = (int)((n_items + 127) / 128);
+    p.splits2 = parts_of((n + tb - 1) / tb, p.rt2, 512);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
+    p.xp = take((int64_t)p.planes * n * p.dp * 2);
+    p.wp = take((int64_t)p.planes * n_items * p.dp * 2);       // not used where the table's rows are operands as they are
+    p.targets = take(n * 4);
+    p.m1 = take((int64_t)p.splits1 * n * 4);
+    p.s1 = take((int64_t)p.splits1 * n * 4);
+    if (grads) {
+        p.o1 = take((int64_t)p.splits1 * n * p.dp * 4);
+        p.init = take(n * 4); p.q = take(n * 4); p.g = take(n * 4);
+        p.s2 = take((int64_t)p.splits2 * n_items * 4);
+        p.o2 = take((int64_t)p.splits2 * n_items * p.dp * 4);
+    }
+    p.bytes = std::max<int64_t>(at, 256);
+    return p;
+}
+
+template <int DP, int PL, int MODE>
+int launch_stream(const StreamArgs &a, hipStream_t st)
+{
+    auto kern = k_stream<DP, PL, 4, MODE>;
+    constexpr int bytes = Shape<DP, PL>::LDS;
+    static_assert(bytes <= 160 * 1024, "a CU's LDS");
+    MF_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.splits * a.row_tiles)), dim3(256), bytes, st, a);
+    MF_LAUNCH_CHECK();
+    return MFSGD_OK;
+}
+
+template <int PL, int MODE>
+int launch_stream_d(int dp, const StreamArgs &a, hipStream_t st)
+{
+    switch (dp) {
+        case 32: return launch_stream<32, PL, MODE>(a, st);
+        case 64: return launch_stream<64, PL, MODE>(a, st);
+        case 128: return launch_stream<128, PL, MODE>(a, st);
+        case 192: return launch_stream<192, PL, MODE>(a, st);
+        default: return launch_stream<256, PL, MODE>(a, st);
+    }
+}
+
+template <typename T, int PL>
+int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *targets, const float *bias, const float *weights, float weight,
+              int64_t n, int64_t n_items, int32_t d, float scale, float *loss, float *lse, T *dx, T *dw, float *db, bool grads, char *ws,
+              hipStream_t st)
+{
+    const LossPlan p = loss_plan(n, n_items, d, PL == 3 ? MFSGD_F32 : MFSGD_BF16, grads);
+    // a bf16 table whose rows are DP wide and start at multiples of 16 bytes is the operand as it is
+    const bool as_is = PL == 1 && d == p.dp && ws_ % 8 == 0 && (uintptr_t)w % 16 == 0;
+    __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
+    int32_t *tg = (int32_t *)(ws + p.targets);
+    auto blocks = [&](int64_t rows) { return dim3((unsigned)((rows * (p.dp / 8) + 255) / 256)); };
+    hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, x, xs, n, d, p.dp, targets, n_items, xp, tg);
+    if (!as_is)
+        hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, w, ws_, n_items, d, p.dp, (const int32_t *)nullptr, n_items, wp,
+                           (int32_t *)nullptr);
+    MF_LAUNCH_CHECK();
+    const __bf16 *items = as_is ? (const __bf16 *)w : wp;
+    const int64_t items_stride = as_is ? ws_ : p.dp, items_plane = n_items * p.dp;
+
+    StreamArgs a = {};
+    a.targets = tg;
+    a.bias = bias;
+    a.c = scale * LOG2E;
+    a.inv_scale = 1.f / scale;
+    a.st = xp; a.st_stride = p.dp; a.st_plane = n * p.dp; a.n_st = n;
+    a.sm = items; a.sm_stride = items_stride; a.sm_plane = items_plane; a.n_sm = n_items;
+    a.splits = p.splits1; a.row_tiles = p.rt1;
+    a.part_m = (float *)(ws + p.m1); a.part_s = (float *)(ws + p.s1); a.part_o = (float *)(ws + p.o1);
+    if (const int rc = grads ? launch_stream_d<PL, LOSS_SUMS>(p.dp, a, st) : launch_stream_d<PL, LOSS>(p.dp, a, st)) return rc;
+
+    JoinArgs j = {};
+    j.n = n; j.n_items = n_items; j.x_stride = xs; j.w_stride = ws_; j.d = d; j.dp = p.dp; j.splits = p.splits1;
+    j.scale = scale; j.weight = weight; j.targets = targets; j.bias = bias; j.weights = weights;
+    j.part_m = a.part_m; j.part_s = a.part_s; j.part_o = a.part_o; j.loss = loss; j.lse = lse;
+    if (grads) {
+        j.row_init = (float *)(ws + p.init); j.row_q = (float *)(ws + p.q);
+        j.row_g = weights ? (float *)(ws + p.g) : nullptr;
+    }
+    hipLaunchKernelGGL((k_join_rows<T>), dim3((unsigned)n), dim3(64), 0, st, j, x, w, dx);
+    MF_LAUNCH_CHECK();
+    if (!grads) return MFSGD_OK;
+
+    a.st = items; a.st_stride = items_stride; a.st_plane = items_plane; a.n_st = n_items;
+    a.sm = xp; a.sm_stride = p.dp; a.sm_plane = n * p.dp; a.n_sm = n;
+    a.splits = p.splits2; a.row_tiles = p.rt2;
+    a.part_m = nullptr; a.part_s = db ? (float *)(ws + p.s2) : nullptr; a.part_o = (float *)(ws + p.o2);
+    a.row_init = j.row_init; a.row_q = j.row_q; a.row_g = j.row_g;
+    if (const int rc = launch_stream_d<PL, TABLE>(p.dp, a, st)) return rc;
+    hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * d + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items, d,
+                       p.dp, scale * weight, weight, dw, db);
+    MF_LAUNCH_CHECK();
+    return MFSGD_OK;
+}
+
+int check_loss(const char *who, const void *x, int64_t xs, const void *w, int64_t ws_, const int32_t *targets, int64_t n, int64_t n_items,
+               int32_t d, float scale, int32_t dtype, const float *loss, const float *lse, void *ws, int64_t ws_bytes, bool grads)
+{
+    MF_ARG(n >= 0 && n <= INT32_MAX / 4 && n_items >= 1 && n_items <= INT32_MAX / 4 && d >= 1 && d <= 256 && xs >= d && ws_ >= d,
+           "%s: bad shape (1 <= d <= 256, at least one item, rows and items below 2^29)", who);
+    MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "%s: unknown dtype %d", who, dtype);
+    MF_ARG(scale > 0 && scale <= 1e30f, "%s: scale must be positive and finite", who);
+    if (n == 0 && !grads) return MFSGD_OK;
+    MF_ARG(w && (n == 0 || (x && targets && loss && lse)), "%s: null pointer", who);
+    const int64_t need = loss_plan(n, n_items, d, dtype, grads).bytes;
+    MF_ARG(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+    return MFSGD_OK;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_zero(T *__restrict__ p, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) store_f32(p + i, 0.f);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads)
+{
+    if (n < 0 || n > INT32_MAX / 4 || n_items < 1 || n_items > INT32_MAX / 4 || d < 1 || d > 256 || (dtype != MFSGD_F32 && dtype != MFSGD_BF16))
+        return -1;
+    return loss_plan(n, n_items, d, dtype, with_grads != 0).bytes;
+}
+
+int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets, const float *bias,
+                           int64_t n, int64_t n_items, int32_t d, float scale, int32_t dtype, float *loss, float *lse, void *workspace,
+                           int64_t workspace_bytes, void *stream)
+{
+    if (const int rc = check_loss("softmax_loss", x, x_stride, table, table_stride, targets, n, n_items, d, scale, dtype, loss, lse, workspace,
+                                  workspace_bytes, false)) return rc;
+    if (n == 0) return MFSGD_OK;
+    if (dtype == MFSGD_F32)
+        return loss_impl<float, 3>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
+                                   loss, lse, nullptr, nullptr, nullptr, false, (char *)workspace, as_stream(stream));
+    return loss_impl<__bf16, 1>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
+                                loss, lse, nullptr, nullptr, nullptr, false, (char *)workspace, as_stream(stream));
+}
+
+int mfsgd_hip_softmax_loss_grads(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets,
+                                 const float *bias, const float *weights, float weight, int64_t n, int64_t n_items, int32_t d, float scale,
+                                 int32_t dtype, float *loss, float *lse, void *dx, void *dtable, float *dbias, void *workspace,
+                                 int64_t workspace_bytes, void *stream)
+{
+    if (const int rc = check_loss("softmax_loss_grads", x, x_stride, table, table_stride, targets, n, n_items, d, scale, dtype, loss, lse, workspace,
+                                  workspace_bytes, true)) return rc;
+    MF_ARG(dtable && (n == 0 || dx), "softmax_loss_grads: null pointer");
+    hipStream_t st = as_stream(stream);
+    if (n == 0) {       // no rows: the table's gradients are zero
+        const unsigned grid = (unsigned)std::min<int64_t>((n_items * d + 255) / 256, 4096);
+        if (dtype == MFSGD_F32) hipLaunchKernelGGL((k_zero<float>), dim3(grid), dim3(256), 0, st, (float *)dtable, n_items * d);
+        else hipLaunchKernelGGL((k_zero<__bf16>), dim3(grid), dim3(256), 0, st, (__bf16 *)dtable, n_items * d);
+        if (dbias) hipLaunchKernelGGL((k_zero<float>), dim3(grid), dim3(256), 0, st, dbias, n_items);
+        MF_LAUNCH_CHECK();
+        return MFSGD_OK;
+    }
+    if (dtype == MFSGD_F32)
+        return loss_impl<float, 3>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
+                                   scale, loss, lse, (float *)dx, (float *)dtable, dbias, true, (char *)workspace, st);
+    return loss_impl<__bf16, 1>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
+                                scale, loss, lse, (__bf16 *)dx, (__bf16 *)dtable, dbias, true, (char *)workspace, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,254 @@
+"""Minibatch operators on factor tables: what a training step over batches needs next to the rating-by-rating kernels.
+
+    embedding           rows of a table by id, scaled                     (beside the implicit term's gather, z = sum y[j] / sqrt N)
+    embedding_grad      its gradient, by sorted tokens
+    softmax_loss        softmax cross entropy against the whole catalogue (beside ExplicitMF.top_n: the same scores, which
+    softmax_loss_grads  ... and its gradients                              are never stored here either)
+    grad_norm           global norm of a set of gradients
+    clip_grads          ... and their clipping by it
+
+The reference has no counterpart: it updates rating by rating.  All arguments are torch ROCm tensors on one device, float32 or
+bfloat16; ids and targets are int32, and a negative one is padding.  Every call runs on the current stream of that device
+without waiting for it, allocates through torch only, and can be captured into a graph.  Results are the same bits on every
+call.  There is no autograd: a gradient is its own call."""
+import torch
+
+from . import _abi
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}       # MFSGD_F32, MFSGD_BF16
+
+
+def _rows(t, name):
+    """(tensor, row stride) of a two-dimensional tensor whose rows are contiguous; others are copied."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name} must be a two-dimensional tensor")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+    n, d = t.shape
+    if d < 1:
+        raise ValueError(f"{name} has rows of no elements")
+    if (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
+        t = t.contiguous()
+    return t, (t.stride(0) if n > 1 else d)
+
+
+def _ids(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor")
+    return t.contiguous()
+
+
+def _vector(t, n, name):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != (n,):
+        raise ValueError(f"{name} must be a float32 tensor of {n} elements")
+    return t.contiguous()
+
+
+class _On:
+    """Makes the tensors' device current for a call and holds its stream; all tensors must be on that one device."""
+
+    def __init__(self, *tensors):
+        _abi.require_gpu()
+        self.device = tensors[0].device
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device != self.device):
+                raise ValueError("all tensors must be on one ROCm device")
+        self.guard = None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        self.stream = torch.cuda.current_stream().cuda_stream
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+    def workspace(self, nbytes):
+        if nbytes < 0:
+            raise ValueError("the batch or the table is too large")
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+
+def _span(t):
+    """Addresses a tensor reaches, or None if it holds nothing."""
+    if t.numel() == 0:
+        return None
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    x, y = _span(a), _span(b)
+    return x is not None and y is not None and x[0] < y[1] and y[0] < x[1]
+
+
+def embedding(table, ids, scale=1.0):
+    """scale * table[ids]: [*ids.shape, d] of the table's type.  A negative id gives a zero row, an id behind the table a row
+    that is not a number."""
+    table, stride = _rows(table, "table")
+    ids = _ids(ids, "ids")
+    n_rows, d = table.shape
+    with _On(table, ids) as on:
+        out = torch.empty((*ids.shape, d), dtype=table.dtype, device=table.device)
+        _abi.check(_abi.lib().mfsgd_hip_embedding(table.data_ptr(), stride, n_rows, d, ids.data_ptr(), ids.numel(), scale,
+                                                  _DTYPES[table.dtype], out.data_ptr(), on.stream))
+    return out
+
+
+def embedding_grad(grad, ids, n_rows, scale=1.0, out=None, accumulate=False):
+    """Gradient of `embedding` for its table: [n_rows, d], row v = scale * the sum of grad's rows whose id is v (in fp32, in the
+    order of ids), zero where no id is v.  `grad` is [*ids.shape, d].  With `out` the result is written there; with
+    `accumulate` it is added to `out` (one gradient of a table used twice; or, with scale = -learning rate, the update of the
+    table itself), whose other rows stay untouched."""
+    if not isinstance(grad, torch.Tensor) or grad.dim() < 1:
+        raise ValueError("grad must be a tensor")
+    ids = _ids(ids, "ids")
+    if tuple(grad.shape[:-1]) != tuple(ids.shape):
+        raise ValueError("grad must be [*ids.shape, d]")
+    n, d, n_rows = ids.numel(), grad.shape[-1], int(n_rows)
+    if n_rows < 0:
+        raise ValueError("n_rows must not be negative")
+    grad, stride = _rows(grad if grad.dim() == 2 else grad.reshape(n, d), "grad")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs an out to add to")
+    else:
+        if not isinstance(out, torch.Tensor) or tuple(out.shape) != (n_rows, d) or out.dtype != grad.dtype:
+            raise ValueError("out must be [n_rows, d] of grad's type")
+        if (d > 1 and out.stride(1) != 1) or (n_rows > 1 and out.stride(0) < d):
+            raise ValueError("out's rows must be contiguous and must not overlap")
+        if _overlap(out, grad) or _overlap(out, ids):
+            raise ValueError("out must not overlap grad or ids")
+    with _On(grad, ids, out) as on:
+        if out is None:
+            out = torch.empty((n_rows, d), dtype=grad.dtype, device=grad.device)
+        ws = on.workspace(_abi.lib().mfsgd_embedding_grad_workspace(n, n_rows, d))
+        _abi.check(_abi.lib().mfsgd_hip_embedding_grad(
+            grad.data_ptr(), stride, ids.data_ptr(), n, n_rows, d, scale, _DTYPES[grad.dtype], 1 if accumulate else 0,
+            out.data_ptr(), out.stride(0) if n_rows > 1 else d, ws.data_ptr(), ws.numel(), on.stream))
+    return out
+
+
+def _loss_args(x, table, targets, bias, scale):
+    x, xs = _rows(x, "x")
+    table, ts = _rows(table, "table")
+    targets = _ids(targets, "targets")
+    n, d = x.shape
+    if table.shape[1] != d or table.dtype != x.dtype:
+        raise ValueError("x and table must have rows of one length and type")
+    if d > 256:
+        raise ValueError("softmax_loss: rows of at most 256 elements")
+    if table.shape[0] < 1:
+        raise ValueError("softmax_loss: the table has no items")
+    if tuple(targets.shape) != (n,):
+        raise ValueError("targets must have an element for every row of x")
+    if not 0 < scale <= 1e30:
+        raise ValueError("scale must be positive and finite")
+    return x, xs, table, ts, targets, _vector(bias, table.shape[0], "bias")
+
+
+def softmax_loss(x, table, targets, bias=None, scale=1.0):
+    """Cross entropy of the softmax over all items: (loss [n], lse [n]) in float32, with the logits
+    z = scale * x @ table.T + bias, lse = logsumexp(z), loss = lse - z[targets].  Rows of at most 256 elements.  A padding row
+    (target < 0) has loss and lse 0 and its x is not looked at; a target behind the table gives a loss that is not a number;
+    a bias of -inf takes an item out of the catalogue."""
+    x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
+    n, d = x.shape
+    with _On(x, table, targets, bias) as on:
+        both = torch.empty((2, n), dtype=torch.float32, device=x.device)
+        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, table.shape[0], d, _DTYPES[x.dtype], 0))
+        _abi.check(_abi.lib().mfsgd_hip_softmax_loss(
+            x.data_ptr(), xs, table.data_ptr(), ts, targets.data_ptr(), None if bias is None else bias.data_ptr(), n,
+            table.shape[0], d, scale, _DTYPES[x.dtype], both.data_ptr(), both.data_ptr() + 4 * n, ws.data_ptr(), ws.numel(),
+            on.stream))
+    return both[0], both[1]
+
+
+def softmax_loss_grads(x, table, targets, bias=None, scale=1.0, weights=1.0):
+    """(loss, lse, dx, dtable, dbias): `softmax_loss` and the gradients of sum(weights * loss).  `weights` is a number or a
+    float32 tensor with an element for every row (1 / n: the mean over n rows).  dx and dtable have the type of x, summed in
+    fp32; dbias is float32, None without a bias."""
+    x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
+    n, d = x.shape
+    n_items = table.shape[0]
+    each = _vector(weights, n, "weights") if isinstance(weights, torch.Tensor) else None
+    with _On(x, table, targets, bias, each) as on:
+        both = torch.empty((2, n), dtype=torch.float32, device=x.device)
+        dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+        dtable = torch.empty((n_items, d), dtype=x.dtype, device=x.device)
+        dbias = None if bias is None else torch.empty(n_items, dtype=torch.float32, device=x.device)
+        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, n_items, d, _DTYPES[x.dtype], 1))
+        _abi.check(_abi.lib().mfsgd_hip_softmax_loss_grads(
+            x.data_ptr(), xs, table.data_ptr(), ts, targets.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if each is None else each.data_ptr(), 1.0 if each is not None else float(weights), n, n_items, d, scale,
+            _DTYPES[x.dtype], both.data_ptr(), both.data_ptr() + 4 * n, dx.data_ptr(), dtable.data_ptr(),
+            None if dbias is None else dbias.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
+    return both[0], both[1], dx, dtable, dbias
+
+
+def _dense(t):
+    """Every element of the storage stretch exactly once, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n != 1):
+        if s != at:
+            return False
+        at *= n
+    return True
+
+
+def _grad_set(tensors, name):
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        raise ValueError(f"{name} is empty")
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
+            raise TypeError(f"{name} must be float32 or bfloat16 tensors")
+        if t.numel() and not _dense(t):
+            raise ValueError(f"{name} must be dense tensors (no gaps, no element twice)")
+    return tensors
+
+
+def _set_args(tensors):
+    n = len(tensors)
+    return ((_abi.c_vp * n)(*[t.data_ptr() for t in tensors]), (_abi.c_i64 * n)(*[t.numel() for t in tensors]),
+            (_abi.c_i32 * n)(*[_DTYPES[t.dtype] for t in tensors]))
+
+
+def grad_norm(tensors):
+    """sqrt of the sum of all squares of all tensors (float32 and bfloat16 in any mix), as a float32 tensor of no dimensions."""
+    tensors = _grad_set(tensors, "tensors")
+    with _On(*tensors) as on:
+        norm = torch.empty((), dtype=torch.float32, device=on.device)
+        ptrs, sizes, dtypes = _set_args(tensors)
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, len(tensors)))
+        _abi.check(_abi.lib().mfsgd_hip_grad_norm(ptrs, sizes, dtypes, len(tensors), norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                  on.stream))
+    return norm
+
+
+def clip_grads(tensors, max_norm, out=None):
+    """Scales all tensors by min(1, max_norm / norm), norm being their global norm, in place or into `out` (tensors of the same
+    shapes, types and strides).  Returns the norm before clipping, without waiting for it."""
+    tensors = _grad_set(tensors, "tensors")
+    if not max_norm > 0:
+        raise ValueError("max_norm must be positive")
+    if out is not None:
+        out = _grad_set(out, "out")
+        if len(out) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.stride() != t.stride()
+                                           for o, t in zip(out, tensors)):
+            raise ValueError("out must have a tensor like each of tensors")
+    with _On(*tensors, *(out or ())) as on:
+        norm = torch.empty((), dtype=torch.float32, device=on.device)
+        ptrs, sizes, dtypes = _set_args(tensors)
+        outs = None if out is None else _set_args(out)[0]
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, len(tensors)))
+        _abi.check(_abi.lib().mfsgd_hip_clip_grads(ptrs, outs, sizes, dtypes, len(tensors), max_norm, norm.data_ptr(),
+                                                   ws.data_ptr(), ws.numel(), on.stream))
+    return norm

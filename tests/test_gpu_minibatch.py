@@ -1,0 +1,484 @@
+"""The minibatch operators on the GPU against their formulas in 64 bits.
+
+Tolerances count roundings (half a step each: u = 2^-24 in fp32, h = eps / 2 of the output's type) and are worked out from
+the formulas, element by element, from the absolute values that are summed."""
+import math
+
+import pytest
+import torch
+
+import recommender_amd as ra
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TINY = 1e-30
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * std).to(dtype)
+
+
+def ids_of(g, n, rows, dtype=torch.int32):
+    return torch.randint(0, max(rows, 1), (n,), device="cuda", generator=g).to(dtype)
+
+
+def close(got, want, tol):
+    got = got.double()
+    assert got.shape == want.shape
+    assert bool(torch.isfinite(got).all())
+    over = ((got - want).abs() - tol).max().item() if got.numel() else -1.0
+    assert over <= 0, f"off by {((got - want).abs() / (tol + TINY)).max().item():.3g} times the tolerance"
+
+
+# ------------------------------------------------------------------ lookup
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, rows, d, pad", [(1, 1, 1, 0), (7, 5, 3, 0), (33, 100, 40, 24), (1000, 37, 100, 0), (257, 1000, 128, 0),
+                                             (64, 20, 129, 1), (5000, 3000, 256, 0), (3, 10, 1000, 6)])
+def test_embedding(dtype, n, rows, d, pad):
+    g = gen(n + d)
+    table = normal(g, rows, d + pad, dtype=dtype)[:, :d]
+    ids = ids_of(g, n, rows)
+    ids[n // 2] = -1
+    if n > 4:
+        ids[1], ids[2] = rows, 2 ** 31 - 1
+    out = ra.embedding(table, ids, scale=1.7)
+    inside = (ids >= 0) & (ids < rows)
+    want = table.double()[ids.long().clamp(0, rows - 1)] * 1.7
+    close(out[inside], want[inside], (half(dtype) + 2 * U) * want[inside].abs())      # 1.7 in fp32, the product, the store
+    assert bool((out[ids < 0] == 0).all()) and bool(torch.isnan(out[ids >= rows].float()).all())
+
+
+def test_embedding_shapes_and_alignment():
+    g = gen(1)
+    base = normal(g, 1 + 50 * 16, dtype=BF16)
+    table = base[1:].view(50, 16)                     # rows that start 2 bytes behind a multiple of 16
+    ids = ids_of(g, 24, 50).view(2, 3, 4)
+    assert torch.equal(ra.embedding(table, ids), table[ids.long()])
+    assert torch.equal(ra.embedding(table.t().contiguous().t(), ids), table[ids.long()])       # columns contiguous
+    assert torch.equal(ra.embedding(table[:1].expand(9, 16), ids % 9), table[:1].expand(2, 3, 4, 16))
+    assert ra.embedding(table, ids[:0]).shape == (0, 3, 4, 16)
+    assert torch.equal(ra.embedding(table, ids.transpose(0, 2)), table[ids.transpose(0, 2).long()])
+
+
+def test_embedding_far_rows():
+    """A table of more than 2^32 bytes and 2^31 elements: offsets in 64 bits."""
+    rows, d = (1 << 23) + 5, 260
+    table = torch.zeros(rows, d, dtype=BF16, device="cuda")
+    ids = torch.tensor([0, 1 << 22, rows - 1, rows - 2], dtype=torch.int32, device="cuda")
+    for k, i in enumerate(ids.tolist()):
+        table[i] = k + 1.0
+    assert torch.equal(ra.embedding(table, ids)[:, 259].float().cpu(), torch.arange(1.0, 5.0))
+    grad = torch.ones(4, d, dtype=BF16, device="cuda")
+    ra.embedding_grad(grad, ids, rows, out=table, accumulate=True)
+    assert torch.equal(table[ids.long(), 259].float().cpu(), torch.arange(2.0, 6.0)) and float(table[5].abs().sum()) == 0
+
+
+# ------------------------------------------------------------------ its gradient
+def grad_want(grad, ids, rows, scale):
+    inside = (ids >= 0) & (ids < rows)
+    at = ids[inside].long()
+    want = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device="cuda")
+    mass = want.clone()
+    want.index_put_((at,), grad.double()[inside] * scale, accumulate=True)
+    mass.index_put_((at,), grad.double()[inside].abs() * abs(scale), accumulate=True)
+    count = torch.bincount(at, minlength=rows).double()[:, None]
+    return want, mass, count
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, rows, d, kind", [
+    (0, 5, 8, "even"), (1, 1, 1, "even"), (1, 7, 40, "even"), (63, 1000, 3, "even"), (64, 10, 100, "even"), (257, 1, 33, "even"),
+    (300, 50, 128, "one"), (1000, 1682, 32, "popular"), (4095, 600, 129, "popular"), (4096, 1024, 64, "one"),
+    (4097, 1023, 64, "popular"), (8192, 1024, 17, "one"), (20000, 17770, 128, "popular"), (30011, 59047, 200, "popular"),
+    (50000, 3, 256, "even"), (5000, 2000003, 4, "even"), (6000, 100, 520, "popular")])
+def test_embedding_grad(dtype, n, rows, d, kind):
+    g = gen(n + rows + d)
+    grad = normal(g, n, d, dtype=dtype)
+    if kind == "one":
+        ids = torch.full((n,), rows // 2, dtype=torch.int32, device="cuda")
+    else:
+        u = torch.rand(n, device="cuda", generator=g, dtype=torch.float64)
+        ids = ((u ** 4 if kind == "popular" else u) * rows).clamp(max=rows - 1).int()
+    if n > 10:
+        ids[3], ids[7], ids[9] = -1, rows, 2 ** 31 - 1
+    want, mass, count = grad_want(grad, ids, rows, -0.75)
+    out = ra.embedding_grad(grad, ids, rows, scale=-0.75)
+    tol = (count + 1) * U * mass * 1.01 + half(dtype) * want.abs()
+    close(out, want, tol)
+    assert bool((out[(count == 0)[:, 0]] == 0).all())
+    assert torch.equal(out, ra.embedding_grad(grad, ids, rows, scale=-0.75))          # the same bits
+    # added to a padded table of its own
+    base = normal(g, rows, d + 5, dtype=dtype)
+    before = base.clone()
+    got = ra.embedding_grad(grad, ids, rows, scale=-0.75, out=base[:, :d], accumulate=True)
+    assert got.data_ptr() == base.data_ptr()
+    full = want + before[:, :d].double()
+    close(got, full, (count + 1) * U * 1.01 * mass + U * full.abs() + half(dtype) * full.abs() + TINY)
+    assert torch.equal(base[:, d:], before[:, d:])                                    # what lies between the rows
+    assert torch.equal(base[(count == 0)[:, 0]], before[(count == 0)[:, 0]])
+
+
+def test_embedding_grad_is_the_lookups():
+    """<dY, lookup(T + e D) - lookup(T - e D)> / 2e = <gradient, D>: the lookup is linear, so the difference has no remainder."""
+    g = gen(3)
+    table, way, grad = normal(g, 90, 24), normal(g, 90, 24), normal(g, 500, 24)
+    ids = ids_of(g, 500, 90)
+    ids[5] = -1
+    up, down = ra.embedding(table + way, ids, 1.5), ra.embedding(table - way, ids, 1.5)
+    left = (grad.double() * (up.double() - down.double())).sum() / 2
+    right = (ra.embedding_grad(grad, ids, 90, 1.5).double() * way.double()).sum()
+    size = (grad.double().abs() * (up.double().abs() + down.double().abs())).sum()
+    assert abs(left - right) <= 40 * U * size
+
+
+# ------------------------------------------------------------------ loss
+def loss_case(g, n, items, d, dtype, bias, spread=2.0):
+    x = normal(g, n, d, dtype=dtype)
+    w = normal(g, items, d, dtype=dtype, std=spread / math.sqrt(d))
+    b = normal(g, items) if bias else None
+    return x, w, ids_of(g, n, items), b
+
+
+def loss_want(x, w, t, b, scale, weights=None):
+    """(loss, lse, dx, dw, db) and the same of absolute values, in 64 bits; rows without a target have no part in it"""
+    n, items = x.shape[0], w.shape[0]
+    x, w = x.double(), w.double()
+    live = (t >= 0) & (t < items)
+    x = torch.where(live[:, None], x, torch.zeros_like(x))
+    z = scale * x @ w.T
+    size = scale * x.abs() @ w.abs().T
+    if b is not None:
+        z, size = z + b.double(), size + b.double().abs()
+    lse = torch.logsumexp(z, 1)
+    at = t.long().clamp(0, items - 1)[:, None]
+    hit = torch.zeros_like(z).scatter_(1, at, 1.0)
+    p = torch.exp(z - lse[:, None])
+    others = (p * (1 - hit)).sum(1, keepdim=True)
+    share = (torch.ones(n, device="cuda", dtype=torch.float64) if weights is None else weights.double().expand(n)) * live
+    gr = torch.where(hit > 0, -others, p) * share[:, None]
+    out = [torch.where(live, lse - z.gather(1, at)[:, 0], 0.0), torch.where(live, lse, 0.0), scale * gr @ w, scale * gr.T @ x, gr.sum(0)]
+    big = gr.abs()
+    return out, [size.where(torch.isfinite(size), torch.zeros_like(size)).amax(1), scale * big @ w.abs(), scale * big.T @ x.abs(), big.sum(0)]
+
+
+def loss_tolerances(out, mass, n, items, d, dtype):
+    """A logit: d products and sums (three bf16 parts leave 3 u of a product) and the steps to and from log2 units, on values
+    up to `size`; a lane's running sum of up to items / 32 terms of which each exponential is off by its argument's error."""
+    size = mass[0]
+    logit = (d + 16) * U * size
+    lse = 2 * logit + (items / 32 + 64) * U + 4 * U * out[1].abs() + 2 * U
+    rel = (2 * lse + logit).max()
+    held = 2.0 ** -8 if dtype == BF16 else 4 * U                # the exponentials as operands of the second product
+    grad = lambda k, terms: (rel + held + (terms + 64) * U) * mass[k - 1] + half(dtype) * out[k].abs() + TINY    # noqa: E731
+    return [2 * lse, 2 * lse, grad(2, items), grad(3, n), (rel + (n + 64) * U) * mass[3] + TINY]
+
+
+LOSS_CASES = [(1, 1, 1), (1, 5, 8), (3, 31, 40), (33, 64, 16), (40, 33, 32), (64, 1000, 64), (129, 257, 100), (200, 700, 128),
+              (31, 2000, 129), (65, 300, 192), (130, 500, 193), (300, 129, 256), (1000, 40, 24)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", LOSS_CASES)
+def test_softmax_loss_and_gradients(dtype, n, items, d):
+    g = gen(n * items + d)
+    bias, scale = (n + d) % 2 == 0, 0.8
+    x, w, t, b = loss_case(g, n, items, d, dtype, bias)
+    if n > 3:
+        t[1], t[n - 1] = -1, -100
+    each = normal(g, n) if n % 2 else None                       # weights of either sign
+    out, mass = loss_want(x, w, t, b, torch.tensor(scale, dtype=F32).double().item(), each)
+    tol = loss_tolerances(out, mass, n, items, d, dtype)
+    loss, lse = ra.softmax_loss(x, w, t, bias=b, scale=scale)
+    close(loss, out[0], tol[0])
+    close(lse, out[1], tol[1])
+    got = ra.softmax_loss_grads(x, w, t, bias=b, scale=scale, weights=1.0 if each is None else each)
+    for k in range(4 if b is None else 5):
+        close(got[k], out[k], tol[k])
+    assert (got[4] is None) == (b is None) and got[2].dtype == dtype and got[3].dtype == dtype
+    again = ra.softmax_loss_grads(x, w, t, bias=b, scale=scale, weights=1.0 if each is None else each)
+    assert all(a is None or torch.equal(a, c) for a, c in zip(got, again))           # the same bits
+    if n > 3:
+        assert float(loss[1]) == 0 and float(lse[1]) == 0 and float(got[2][1].abs().sum()) == 0
+
+
+def test_softmax_loss_many_items_and_rows():
+    """Several parts of either axis, joined."""
+    for n, items, d, dtype in ((70, 60000, 64, BF16), (5000, 300, 128, BF16), (2, 100000, 128, F32), (4100, 4099, 40, F32)):
+        x, w, t, b = loss_case(gen(items), n, items, d, dtype, True)
+        out, mass = loss_want(x, w, t, b, 1.0, torch.tensor(1.0 / n, dtype=F32).cuda())
+        tol = loss_tolerances(out, mass, n, items, d, dtype)
+        got = ra.softmax_loss_grads(x, w, t, bias=b, weights=1.0 / n)
+        for k in range(5):
+            close(got[k], out[k], tol[k])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_softmax_loss_masks(dtype):
+    g = gen(8)
+    n, items, d = 70, 300, 48
+    x, w, t, b = loss_case(g, n, items, d, dtype, True)
+    out_of = torch.rand(items, device="cuda", generator=g) < 0.4
+    out_of[64:128] = True                                         # a whole tile
+    b[out_of] = -math.inf
+    out_of[7], b[7] = True, torch.finfo(F32).min                  # the type's lowest value
+    kept = torch.nonzero(~out_of)[:, 0]
+    t = kept[t.long() % len(kept)].int()
+    t[5] = -1
+    x[5] = math.nan                                               # padding is not looked at
+    want_b = torch.where(out_of, torch.full_like(b, -math.inf), b)
+    out, mass = loss_want(x, w, t, want_b, 1.0)
+    tol = loss_tolerances(out, mass, n, items, d, dtype)
+    got = ra.softmax_loss_grads(x, w, t, bias=b)
+    for k in range(5):
+        close(got[k], out[k], tol[k])
+    assert float(got[3][out_of].abs().sum()) == 0 and float(got[4][out_of].abs().sum()) == 0
+    assert torch.equal(ra.softmax_loss(x, w, t, bias=b)[0], got[0])
+    # a target that is out of the catalogue, one behind the table
+    t2 = t.clone()
+    t2[0], t2[1] = int(torch.nonzero(out_of)[0]), items
+    loss, lse, dx, dw, db = ra.softmax_loss_grads(x, w, t2, bias=b)
+    assert math.isinf(float(loss[0])) and float(loss[0]) > 0 and math.isfinite(float(lse[0]))
+    assert math.isnan(float(loss[1])) and float(dx[1].abs().sum()) == 0
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())
+    assert abs(float(db[t2[0]]) + 1.0) < 1e-5
+    # nothing in the catalogue
+    loss, lse, dx, dw, db = ra.softmax_loss_grads(x, w, t, bias=torch.full_like(b, -math.inf))
+    live = t >= 0
+    assert bool((loss[live] == math.inf).all()) and bool((lse[live] == -math.inf).all())
+    assert float(dx.abs().sum()) == 0 and float(dw.abs().sum()) == 0 and float(db.abs().sum()) == 0
+
+
+def test_softmax_loss_not_a_number_shows():
+    x, w, t, b = loss_case(gen(9), 40, 100, 32, F32, True)
+    x[3, 4] = math.nan
+    loss, lse = ra.softmax_loss(x, w, t, bias=b)
+    assert bool(torch.isnan(loss[3])) and bool(torch.isnan(lse[3]))
+    others = torch.arange(40, device="cuda") != 3
+    assert bool(torch.isfinite(loss[others]).all())
+    w[50, 2] = math.inf
+    assert not bool(torch.isfinite(ra.softmax_loss(x, w, t, bias=b)[0]).any())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_softmax_loss_learnt_rows(dtype):
+    """Targets that hold nearly the whole probability: loss and gradient keep their digits."""
+    n, items, d = 64, 200, 64
+    g = gen(10)
+    t = ids_of(g, n, items)
+    w = normal(g, items, d, dtype=dtype)
+    x = (w[t.long()].float() * 0.35).to(dtype)                    # the target's logit lies about 0.35 d = 22 above the others
+    out, mass = loss_want(x, w, t, None, 1.0)
+    tol = loss_tolerances(out, mass, n, items, d, dtype)
+    got = ra.softmax_loss_grads(x, w, t)
+    # here the loss itself is small, and its error relative to it: the others' share times the error of their logits
+    rel = 4 * (d + 16) * U * mass[0].max() + (items / 32 + 64) * U
+    close(got[0], out[0], rel * out[0] + TINY)
+    close(got[2], out[2], tol[2])
+    close(got[3], out[3], tol[3])
+
+
+def test_softmax_loss_large_logits():
+    """Logits of some thousand, rising along the items: the running maximum moves all the time."""
+    n, items, d = 33, 900, 32
+    x = torch.ones(n, d, device="cuda")
+    w = torch.arange(items, device="cuda", dtype=F32)[:, None].expand(items, d) / 8
+    w = w.contiguous()
+    t = torch.arange(n, device="cuda", dtype=torch.int32) * 27
+    for way in (w, w.flip(0).contiguous()):
+        out, mass = loss_want(x, way, t, None, 1.0)
+        tol = loss_tolerances(out, mass, n, items, d, F32)
+        got = ra.softmax_loss_grads(x, way, t)
+        for k in range(4):
+            close(got[k], out[k], tol[k])
+
+
+def test_softmax_loss_strides():
+    g = gen(11)
+    n, items, d = 37, 90, 64
+    wide = normal(g, items, 96, dtype=BF16)
+    xs = normal(g, n, 70, dtype=BF16)
+    t = ids_of(g, n, items)
+    want = ra.softmax_loss_grads(xs[:, :d].contiguous(), wide[:, :d].contiguous(), t)
+    got = ra.softmax_loss_grads(xs[:, :d], wide[:, :d], t)
+    assert all(torch.equal(a, b) for a, b in zip(got[:4], want[:4]))
+    odd = normal(g, 1 + items * d, dtype=BF16)[1:].view(items, d).copy_(wide[:, :d])       # not at a multiple of 16 bytes
+    got = ra.softmax_loss_grads(xs[:, :d].t().contiguous().t(), odd, t)
+    assert all(torch.equal(a, b) for a, b in zip(got[:4], want[:4]))
+    none = ra.softmax_loss_grads(xs[:0, :d], wide[:, :d], t[:0])
+    assert none[0].shape == (0,) and none[2].shape == (0, d) and float(none[3].abs().sum()) == 0
+
+
+def test_softmax_gradients_against_differences():
+    """d/de of the 64-bit loss at x + e u, w + e v, b + e c, by central differences, is <dx, u> + <dw, v> + <db, c>."""
+    g = gen(12)
+    n, items, d = 50, 170, 40
+    x, w, t, b = loss_case(g, n, items, d, F32, True, spread=1.0)
+    t[4] = -1
+    each = normal(g, n)
+    _, _, dx, dw, db = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+    u, v, c = normal(g, n, d), normal(g, items, d), normal(g, items)
+
+    def total(e):
+        out, _ = loss_want(x.double() + e * u.double(), w.double() + e * v.double(), t, b.double() + e * c.double(), 1.0)
+        return float((out[0] * each.double()).sum())
+    e = 1e-4
+    slope = (total(e) - total(-e)) / (2 * e)
+    wider = (total(2 * e) - total(-2 * e)) / (4 * e)
+    said = sum(float((a.double() * k.double()).sum()) for a, k in ((dx, u), (dw, v), (db, c)))
+    out, mass = loss_want(x, w, t, b, 1.0, each)
+    tol = loss_tolerances(out, mass, n, items, d, F32)
+    room = sum(float((tol[k] * y.abs()).sum()) for k, y in ((2, u), (3, v), (4, c)))
+    assert abs(said - slope) <= room + abs(wider - slope)         # the remainder is a third of what doubling e changes
+
+
+# ------------------------------------------------------------------ norm and clipping
+SETS = [[(1,)], [(5,), (0,), (3, 7)], [(4096,), (4097,), (12289,)], [(6040, 64), (3706, 64), (6040,), (3706,)],
+        [(i % 7,) for i in range(300)], [(3000, 1000), (11,)]]
+
+
+@pytest.mark.parametrize("shapes", SETS, ids=lambda s: f"{len(s)}x{s[0]}")
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mixed"])
+def test_clip(shapes, kind):
+    g = gen(len(shapes))
+    types = {"f32": [F32], "bf16": [BF16], "mixed": [F32, BF16]}[kind]
+    grads = [normal(g, *s, dtype=types[i % len(types)]) for i, s in enumerate(shapes)]
+    norm = math.sqrt(sum(float((t.double() ** 2).sum()) for t in grads))
+    assert abs(float(ra.grad_norm(grads)) - norm) <= 4 * U * norm               # float64 sums, rounded once
+    for top in (0.25 * norm, 4 * norm):
+        want = [t.double() * min(1.0, top / norm) for t in grads]
+        out = [torch.full_like(t, math.nan) for t in grads]
+        keep = [t.clone() for t in grads]
+        assert abs(float(ra.clip_grads(grads, top, out=out)) - norm) <= 4 * U * norm
+        for t, k, o, x in zip(grads, keep, out, want):
+            assert torch.equal(t, k)
+            if t.numel():
+                close(o, x, (half(t.dtype) + 8 * U) * x.abs())
+        place = [t.clone() for t in grads]
+        ra.clip_grads(place, top)
+        assert all(torch.equal(a, b) for a, b in zip(place, out))
+
+
+def test_clip_views_and_odd_addresses():
+    g = gen(20)
+    base = normal(g, 40000)
+    parts = [base[1:10001], base[10003:20000].view(13, 769), base[20001:20002], base[30000:39999:1].view(99, 101).t()]
+    before = base.clone()
+    norm = math.sqrt(sum(float((p.double() ** 2).sum()) for p in parts))
+    ra.clip_grads(parts, norm / 2)
+    moved = torch.zeros(40000, dtype=torch.bool, device="cuda")
+    for a, z in ((1, 10001), (10003, 20000), (20001, 20002), (30000, 39999)):
+        moved[a:z] = True
+    assert torch.equal(base[~moved], before[~moved])
+    close(base[moved], before[moved].double() / 2, 10 * U * before[moved].double().abs())
+
+
+def test_clip_extremes():
+    for value in (1e30, 1e-30):                                  # squares that fp32 cannot hold
+        t = torch.full((1000,), value, device="cuda")
+        norm = value * math.sqrt(1000)
+        assert abs(float(ra.grad_norm([t])) / norm - 1) < 1e-5
+        ra.clip_grads([t], norm / 10)
+        assert abs(float(t[7]) / value * 10 - 1) < 1e-5
+    t = torch.zeros(10, device="cuda")
+    assert float(ra.clip_grads([t], 1.0)) == 0 and float(t.abs().sum()) == 0
+    t = torch.ones(10, device="cuda")
+    t[3] = math.inf
+    assert math.isinf(float(ra.clip_grads([t], 1.0))) and float(t[0]) == 0 and math.isnan(float(t[3]))
+    t = torch.ones(10, device="cuda")
+    t[3] = math.nan
+    assert math.isnan(float(ra.clip_grads([t], 1.0))) and bool(torch.isnan(t).all())
+    assert float(ra.grad_norm([torch.empty(0, device="cuda")])) == 0
+    t = torch.ones(8, device="cuda")
+    with pytest.raises(Exception, match="shares memory"):
+        ra.clip_grads([t, t[4:]], 1.0)
+
+
+# ------------------------------------------------------------------ together
+def step_want(users, items, P, Q, b, lr, top, scale):
+    n = len(users)
+    P, Q, b = P.double(), Q.double(), b.double()
+    out, _ = loss_want(P[users.long()], Q, items, b, scale, torch.tensor(1.0 / n).cuda())
+    dP = torch.zeros_like(P).index_add_(0, users.long(), out[2])
+    norm = math.sqrt(sum(float((t ** 2).sum()) for t in (dP, out[3], out[4])))
+    f = lr * min(1.0, top / norm)
+    return out[0], norm, P - f * dP, Q - f * out[3], b - f * out[4]
+
+
+def batch(seed, n=600, users=90, items=700, d=40):
+    g = gen(seed)
+    P, Q, b = normal(g, users, d), normal(g, items, d), normal(g, items)
+    u, i = ids_of(g, n, users), ids_of(g, n, items)
+    i[3] = -1
+    return u, i, P, Q, b
+
+
+def test_ranking_step():
+    u, i, P, Q, b = batch(30)
+    want = step_want(u, i, P, Q, b, 0.5, 0.05, 0.3)
+    loss, norm = ra.ExplicitMF.ranking_step(u, i, P, Q, b, lr=0.5, max_norm=0.05, scale=0.3)
+    # fp32 throughout: gradients to 1e-5 of the largest (some hundred roundings), the step is lr times them
+    assert abs(float(norm) / want[1] - 1) < 1e-5
+    close(loss, want[0], 1e-5 + torch.zeros_like(want[0]))
+    for got, x in ((P, want[2]), (Q, want[3]), (b, want[4])):
+        close(got, x, 2 * U * x.abs() + 0.5 * 0.05 * 1e-5)
+
+
+def test_captured_step_replays():
+    """The whole step in a graph, replayed on new inputs with eager work of the same kind in between."""
+    u, i, P, Q, b = batch(31, n=5000)
+    keep = [t.clone() for t in (P, Q, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ra.ExplicitMF.ranking_step(u, i, P, Q, b, max_norm=0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, norm = ra.ExplicitMF.ranking_step(u, i, P, Q, b, max_norm=0.1)
+    for seed in (32, 33, 34, 35):
+        u2, i2, *_ = batch(seed, n=5000)
+        u.copy_(u2)
+        i.copy_(i2)
+        for t, k in zip((P, Q, b), keep):
+            t.copy_(k)
+        graph.replay()
+        mine = [k.clone() for k in keep]
+        loss2, norm2 = ra.ExplicitMF.ranking_step(u2, i2, *mine, max_norm=0.1)
+        torch.cuda.synchronize()
+        assert torch.equal(loss, loss2) and torch.equal(norm, norm2)
+        assert all(torch.equal(a, c) for a, c in zip((P, Q, b), mine))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have a workspace each."""
+    g = gen(36)
+    sets = [loss_case(g, 300, 5000, 64, BF16, True) for _ in range(2)]
+    grads = [(normal(g, 20000, 32), ids_of(g, 20000, 500)) for _ in range(2)]
+    want = [(ra.softmax_loss_grads(x, w, t, bias=b), ra.embedding_grad(*e, 500)) for (x, w, t, b), e in zip(sets, grads)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for s, (x, w, t, b), e in zip(streams, sets, grads):
+            with torch.cuda.stream(s):
+                got.append((ra.softmax_loss_grads(x, w, t, bias=b), ra.embedding_grad(*e, 500)))
+        torch.cuda.synchronize()
+        for (a, e), (c, f) in zip(got, want):
+            assert all(torch.equal(y, z) for y, z in zip(a, c)) and torch.equal(e, f)
+
+
+def test_one_device():
+    with pytest.raises(ValueError, match="one ROCm device"):
+        ra.embedding(torch.zeros(3, 4, device="cuda"), torch.zeros(2, dtype=torch.int32))
