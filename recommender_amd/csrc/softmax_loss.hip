@@ -54,28 +54,48 @@ struct StreamArgs {
     const float *row_init, *row_q, *row_g;   // pass 2: -lse / scale, g (1 - p_t), g (g: the row's weight, NULL: all 1)
 };
 
-template <int DP, int PL> struct Shape {
+// UT: 32-row tiles of stationary rows a wave keeps.
+template <int DP, int PL, int MODE> struct Shape {
+#ifndef UTX
+#define UTX (PL == 3 || (MODE != LOSS && DP > 128) ? 1 : 2)
+#endif
+#ifndef RX
+#define RX 40
+#endif
+    static constexpr int UT = UTX;
     static constexpr int TB = (PL == 3 && DP > 32) ? 32 : 64;        // streamed rows a tile
     static constexpr int CH = DP / 8;                                // 16-byte pieces of a row
     static constexpr int BUF = PL * TB * DP * 2;                     // bytes of a tile
-    static constexpr int LDS = 2 * BUF + 2 * TB * 12;
+    static constexpr int LDS = 2 * BUF + 2 * TB * 16;
+    // registers: the stationary rows, the sums, the logits and what is in flight; two waves a SIMD have 256 each
+    static constexpr int REGS = UT * PL * DP / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + RX;
+    static constexpr int WAVES = REGS <= 256 ? 2 : 1;
 };
 
-// piece c of row r lies at piece c ^ swizzle(r): the 8 rows that a read touches at once then lie in different banks
-template <int CH> __device__ __forceinline__ int swizzle(int r) { return CH >= 8 ? (r & 7) : ((r >> 1) & 3); }
-
-template <int DP, int PL, int NW, int MODE>
-__global__ __launch_bounds__(NW * 64, (DP * PL > 256 ? 1 : 2)) void k_stream(const StreamArgs a)
+// Piece c of row r lies at piece c ^ swizzle(r).  The logits' operand takes one piece of 16 consecutive rows at a time, the
+// transposed operand four neighbouring pieces of 4 consecutive rows: either set has to cover the 64 banks once.
+template <int CH> __device__ __forceinline__ int swizzle(int r)
 {
-    using S = Shape<DP, PL>;
-    constexpr int TB = S::TB, CH = S::CH, BUF = S::BUF, KS = DP / 16, DT = DP / 32;
-    constexpr int Q = BUF / (NW * 1024);
-    static_assert(BUF % (NW * 1024) == 0, "a tile is a whole number of 1 KB pieces per wave");
+    if constexpr (CH % 16 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (CH % 8 == 0) return ((r & 3) << 1) | ((r >> 2) & 1);
+    else return (r & 2) | ((r >> 2) & 1);
+}
+
+template <int DP, int PL, int MODE>
+__global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(const StreamArgs a)
+{
+    using S = Shape<DP, PL, MODE>;
+    constexpr int UT = S::UT, TB = S::TB, CH = S::CH, BUF = S::BUF, KS = DP / 16, DT = DP / 32, PLANE = TB * DP * 2;
+    constexpr int Q = BUF / 4096;
+#ifndef SCHED
+#define SCHED 4
+#endif
+    static_assert(BUF % 4096 == 0, "a tile is a whole number of 1 KB pieces per wave");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *l_init = (float *)(lds + 2 * BUF);           // [2][TB]
-    float *l_g = l_init + 2 * TB;
-    int32_t *l_t = (int32_t *)(l_g + 2 * TB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, kh = lane >> 5;
+    float *l_g = l_init + 2 * TB, *l_q = l_g + 2 * TB;
+    int32_t *l_t = (int32_t *)(l_q + 2 * TB);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, kh = lane >> 5;
 
     // consecutive workgroups go round the 8 XCDs: the row tiles that walk the same part of the streamed axis share one's L2
     int split, rt;
@@ -87,206 +107,279 @@ __global__ __launch_bounds__(NW * 64, (DP * PL > 256 ? 1 : 2)) void k_stream(con
         split = blockIdx.x / a.row_tiles;
         rt = blockIdx.x % a.row_tiles;
     }
-    const int64_t st0 = ((int64_t)rt * NW + wave) * 32;
-    const int64_t st_row = std::min<int64_t>(st0 + col, a.n_st - 1);
-    const int64_t tiles = (a.n_sm + TB - 1) / TB;
-    const int64_t t0 = tiles * split / a.splits, t1 = tiles * (split + 1) / a.splits;
+    const int32_t n_st = (int32_t)a.n_st, n_sm = (int32_t)a.n_sm;            // both below 2^29
+    const int32_t st0 = (rt * 4 + wave) * (32 * UT);
+    const int32_t tiles = (n_sm + TB - 1) / TB;
+    const int32_t t0 = (int32_t)((int64_t)tiles * split / a.splits), t1 = (int32_t)((int64_t)tiles * (split + 1) / a.splits);
 
-    bf16x8 b[PL][KS];
+    bf16x8 b[UT][PL][KS];
+    int32_t target[UT];
+    float b2[UT];
 #pragma unroll
-    for (int p = 0; p < PL; ++p)
+    for (int u = 0; u < UT; ++u) {
+        const int32_t row = std::min(st0 + 32 * u + col, n_st - 1);
+        target[u] = MODE == TABLE ? -1 : a.targets[row];
+        b2[u] = (MODE == TABLE && a.bias) ? a.bias[row] * LOG2E : 0.f;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-            b[p][s] = *(const bf16x8 *)(a.st + p * a.st_plane + st_row * a.st_stride + 16 * s + 8 * kh);
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                b[u][p][s] = *(const bf16x8 *)(a.st + p * a.st_plane + row * a.st_stride + 16 * s + 8 * kh);
+    }
 
-    auto stage = [&](int64_t t, int buf) {
+    // A tile goes straight from memory to LDS, 1 KB a wave and instruction; its place is the lane's, so the swizzle is in
+    // which piece a lane asks for.
+    constexpr int STEP = 256 / CH;                      // rows an instruction of the whole workgroup covers
+    constexpr bool EVEN = 256 % CH == 0;
+    int32_t from[2];                                    // a lane's offset in the rows of even and odd steps
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const int slot = (q * NW + wave) * 64 + lane;
-            const int p = slot / (TB * CH), r = slot / CH % TB, c = (slot % CH) ^ swizzle<CH>(slot / CH % TB);
-            const int64_t row = std::min<int64_t>(t * TB + r, a.n_sm - 1);
-            __builtin_amdgcn_global_load_lds((const GLB_AS void *)(a.sm + p * a.sm_plane + row * a.sm_stride + c * 8),
-                                             (LDS_AS void *)(lds + buf * BUF + (q * NW + wave) * 1024), 16, 0, 0);
+    for (int v = 0; v < 2; ++v) from[v] = (tid / CH) * (int32_t)a.sm_stride + ((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 8;
+    auto stage = [&](int32_t t, int buf) {
+        const __bf16 *base = a.sm + (int64_t)t * TB * a.sm_stride;
+        const int32_t last = std::min(TB, n_sm - t * TB) - 1;
+        if (EVEN && last == TB - 1) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                constexpr int PER = Q / PL;
+                const __bf16 *rows = base + (q / PER) * a.sm_plane + (q % PER) * STEP * a.sm_stride;
+                __builtin_amdgcn_global_load_lds((const GLB_AS void *)(rows + from[q % PER % 2]),
+                                                 (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {                                        // rows behind the last one are the last one, masked below
+#pragma unroll 1
+            for (int q = 0; q < Q; ++q) {
+                const int slot = q * 256 + tid;
+                const int p = slot / (TB * CH), r = slot / CH % TB, c = (slot % CH) ^ swizzle<CH>(slot / CH % TB);
+                __builtin_amdgcn_global_load_lds((const GLB_AS void *)(base + p * a.sm_plane + std::min(r, last) * a.sm_stride + c * 8),
+                                                 (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
+            }
         }
         if (tid < TB) {
-            const int64_t row = t * TB + tid;
-            const bool in = row < a.n_sm;
-            const int64_t rr = in ? row : a.n_sm - 1;
+            const bool in = tid <= last;
+            const int32_t row = t * TB + std::min(tid, last);
             if constexpr (MODE == TABLE) {
-                l_init[buf * TB + tid] = in ? a.row_init[rr] : -INFINITY;
-                if (a.row_g) l_g[buf * TB + tid] = a.row_g[rr];
-                l_t[buf * TB + tid] = in ? a.targets[rr] : -1;
+                l_init[buf * TB + tid] = in ? a.row_init[row] : -INFINITY;
+                if (a.row_g) l_g[buf * TB + tid] = a.row_g[row];
+                l_q[buf * TB + tid] = a.row_q[row];
+                l_t[buf * TB + tid] = in ? a.targets[row] : -1;
             } else
-                l_init[buf * TB + tid] = in ? (a.bias ? a.bias[rr] * a.inv_scale : 0.f) : -INFINITY;
+                l_init[buf * TB + tid] = in ? (a.bias ? a.bias[row] * a.inv_scale : 0.f) : -INFINITY;
         }
     };
 
-    f32x16 o[MODE == LOSS ? 1 : DT];
+    f32x16 o[UT][MODE == LOSS ? 1 : DT];
+    float m[UT], sum[UT];
 #pragma unroll
-    for (auto &v : o) v = (f32x16)(0.f);
-    float m = -INFINITY, sum = 0.f;
-    const int32_t target = MODE == TABLE ? -1 : a.targets[st_row];
-    const float b2 = (MODE == TABLE && a.bias) ? a.bias[st_row] * LOG2E : 0.f;
+    for (int u = 0; u < UT; ++u) {
+        m[u] = -INFINITY;
+        sum[u] = 0.f;
+#pragma unroll
+        for (auto &v : o[u]) v = (f32x16)(0.f);
+    }
+
+    // LDS addresses of this lane, for the tile in work: the swizzle makes an operand's address no linear function of its
+    // column, but one of 2, 4 or 8 registers and a constant
+    constexpr int NA = CH % 16 == 0 ? 8 : CH % 8 == 0 ? 4 : 2, NT = NA / 2;
+    const LDS_AS char *l3 = (const LDS_AS char *)lds;
+    uint32_t at_a[NA], at_t[NT][2], at_i = 2 * BUF + 16 * kh;
+    const int i16 = lane & 15, half = (lane >> 4) & 1, tr = 4 * kh + (i16 >> 2);
+#pragma unroll
+    for (int s = 0; s < NA; ++s) at_a[s] = col * DP * 2 + ((2 * s + kh) ^ swizzle<CH>(col)) * 16;
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            at_t[d][h] = (tr + 8 * h) * DP * 2 + ((4 * d + 2 * half + ((i16 & 3) >> 1)) ^ swizzle<CH>(tr + 8 * h)) * 16 + (i16 & 1) * 8;
 
     if (t0 < t1) stage(t0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int64_t t = t0; t < t1; ++t) {
-        const int buf = (int)((t - t0) & 1);
+    for (int32_t t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
-        const char *tile = lds + buf * BUF;
-#pragma unroll 1
+#pragma unroll
         for (int sub = 0; sub < TB / 32; ++sub) {
-            // logits (in units of scale) of 32 streamed rows: acc[j] is row 8 (j / 4) + 4 kh + j % 4 for stationary row `col`
-            f32x16 acc;
+            // logits (in units of scale) of 32 streamed rows: acc[u][j] is row 8 (j / 4) + 4 kh + j % 4 for stationary row `col`
+            f32x16 acc[UT];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 v = *(const f32x4 *)(l_init + buf * TB + sub * 32 + 8 * j + 4 * kh);
+                const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (sub * 32 + 8 * j) * 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[4 * j + i] = v[i];
+                for (int i = 0; i < 4; ++i) acc[0][4 * j + i] = v[i];
             }
-            const char *arow = tile + (sub * 32 + col) * DP * 2;
-            const int sw = swizzle<CH>(col);
+#pragma unroll
+            for (int u = 1; u < UT; ++u) acc[u] = acc[0];
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 bf16x8 x[PL];
 #pragma unroll
-                for (int p = 0; p < PL; ++p) x[p] = *(const bf16x8 *)(arow + p * TB * DP * 2 + ((2 * s + kh) ^ sw) * 16);
-                if constexpr (PL == 3) {
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], b[0][s], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[2][s], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[1][s], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[0][s], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[1][s], acc, 0, 0, 0);
+                for (int p = 0; p < PL; ++p) x[p] = *(const LDS_AS bf16x8 *)(l3 + at_a[s % NA] + (sub * 32 * DP * 2 + p * PLANE + s / NA * NA * 32));
+#pragma unroll
+                for (int u = 0; u < UT; ++u) {
+                    if constexpr (PL == 3) {
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], b[u][0][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][2][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[u][1][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[u][0][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][1][s], acc[u], 0, 0, 0);
+                    }
+                    acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][0][s], acc[u], 0, 0, 0);
                 }
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[0][s], acc, 0, 0, 0);
+                if (s % SCHED == SCHED - 1) __builtin_amdgcn_sched_barrier(0);
             }
-            float e[16];
+            bf16x8 w[UT][2][PL];       // the exponentials as operands: j 0..7 and 8..15
+            uint32_t hits = 0, at = 0;
             if constexpr (MODE != TABLE) {
-                float top = acc[0];
+                float top[UT];
+                bool rise = false;
 #pragma unroll
-                for (int j = 1; j < 16; ++j) top = fmaxf(top, acc[j]);
-                const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.c;
-                const bool rise = top > m + SLACK;
+                for (int u = 0; u < UT; ++u) {
+                    float v = acc[u][0];
+#pragma unroll
+                    for (int j = 1; j < 16; ++j) v = fmaxf(v, acc[u][j]);
+                    const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+                    top[u] = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.c;
+                    rise |= top[u] > m[u] + SLACK;
+                }
                 if (__ballot(rise)) {
-                    const float f = rise ? __builtin_amdgcn_exp2f(m - top) : 1.f;    // the first tile: exp2(-inf) = 0
-                    if (rise) m = top;
-                    sum *= f;
-                    if constexpr (MODE == LOSS_SUMS) {
 #pragma unroll
-                        for (auto &v : o) v *= f;
+                    for (int u = 0; u < UT; ++u) {
+                        const bool mine = top[u] > m[u] + SLACK;
+                        const float f = mine ? __builtin_amdgcn_exp2f(m[u] - top[u]) : 1.f;    // the first tile: exp2(-inf) = 0
+                        if (mine) m[u] = top[u];
+                        sum[u] *= f;
+                        if constexpr (MODE == LOSS_SUMS) {
+#pragma unroll
+                            for (auto &v : o[u]) { v *= f; __builtin_amdgcn_sched_barrier(0); }
+                        }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[j], a.c, -ref));
-                const uint32_t at = (uint32_t)(target - (int32_t)(t * TB + sub * 32));
-                if (__ballot(at < 32u)) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) e[j] = at == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
-                }
-                float s4[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);
-                sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
             } else {
+                // rows of the tile whose target is one of this wave's items
+                at = (uint32_t)(l_t[buf * TB + sub * 32 + col] - st0);
+                hits = (uint32_t)__ballot(at < 32u * UT);
+            }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[j], a.c, b2));
-                if (a.row_g) {
+            for (int u = 0; u < UT; ++u) {
+                float e[16];
+                if constexpr (MODE != TABLE) {
+                    const float ref = m[u] == -INFINITY ? 0.f : m[u];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const f32x4 v = *(const f32x4 *)(l_g + buf * TB + sub * 32 + 8 * j + 4 * kh);
+                    for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, -ref));
+                    const uint32_t own = (uint32_t)(target[u] - (t * TB + sub * 32));
+                    if (__ballot(own < 32u)) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) e[4 * j + i] *= v[i];
+                        for (int j = 0; j < 16; ++j) e[j] = own == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, b2[u]));
+                    if (a.row_g) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (2 * TB + sub * 32 + 8 * j) * 4);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) e[4 * j + i] *= v[i];
+                        }
+                    }
+                    if (hits) {             // the target: -g (1 - p_t) in the place of g p_t
+                        uint32_t mine = 0;  // rows of the 32 whose target is this lane's item
+                        for (uint32_t h = hits; h; h &= h - 1) {
+                            const int r = __builtin_ctz(h);
+                            mine |= (uint32_t)(__builtin_amdgcn_readlane((int)at, r) == 32 * u + col) << r;
+                        }
+                        mine >>= 4 * kh;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (4 * TB + sub * 32 + 8 * j) * 4);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) e[4 * j + i] = (mine >> (8 * j + i)) & 1 ? -v[i] : e[4 * j + i];
+                        }
                     }
                 }
-                // rows of the tile whose target is one of this wave's items: -g (1 - p_t) in the place of g p_t
-                const uint32_t at = (uint32_t)(l_t[buf * TB + sub * 32 + col] - (int32_t)st0);
-                uint32_t hits = (uint32_t)__ballot(at < 32u);
-                while (hits) {
-                    const int r = __builtin_ctz(hits);
-                    hits &= hits - 1;
-                    const int item = __builtin_amdgcn_readlane((int)at, r);
-                    const float g = -a.row_q[t * TB + sub * 32 + r];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) e[j] = (r == 8 * (j / 4) + 4 * kh + j % 4 && col == item) ? g : e[j];
-                }
-                if (a.part_s) {
+                if (MODE != TABLE || a.part_s) {
                     float s4[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);
-                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    sum[u] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                }
+                if constexpr (MODE != LOSS) {
+#pragma unroll
+                    for (int p = 0; p < PL; ++p)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                v[q] = pack_bf16(e[8 * k + 2 * q], e[8 * k + 2 * q + 1]);
+                                if (p + 1 < PL) { e[8 * k + 2 * q] -= bf16_lo(v[q]); e[8 * k + 2 * q + 1] -= bf16_hi(v[q]); }
+                            }
+                            w[u][k][p] = __builtin_bit_cast(bf16x8, *(const uint4 *)v);
+                        }
                 }
             }
             if constexpr (MODE != LOSS) {
-                // o[dt][j] += sum over the 32 streamed rows of their column 32 dt + 8 (j / 4) + 4 kh + j % 4 times e
-                const int i = lane & 15, g = (lane >> 4) & 1;
+                // o[u][dt][j] += sum over the 32 streamed rows of their column 32 dt + 8 (j / 4) + 4 kh + j % 4 times e
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    bf16x8 w[PL];
-                    {
-                        float rest[8];
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) rest[q] = e[8 * k + q];
-#pragma unroll
-                        for (int p = 0; p < PL; ++p) {
-                            uint32_t u[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                u[q] = pack_bf16(rest[2 * q], rest[2 * q + 1]);
-                                if (p + 1 < PL) { rest[2 * q] -= bf16_lo(u[q]); rest[2 * q + 1] -= bf16_hi(u[q]); }
-                            }
-                            w[p] = __builtin_bit_cast(bf16x8, *(const uint4 *)u);
-                        }
-                    }
-                    const int r = sub * 32 + 16 * k + 4 * kh + (i >> 2);        // and r + 8: the same swizzle
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const int piece = (4 * dt + 2 * g + ((i & 3) >> 1)) ^ swizzle<CH>(r);
                         bf16x8 x[PL];
 #pragma unroll
                         for (int p = 0; p < PL; ++p) {
-                            const char *src = tile + p * TB * DP * 2 + r * DP * 2 + piece * 16 + (i & 1) * 8;
-                            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)src);
-                            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(src + 8 * DP * 2));
+                            const int imm = (sub * 32 + 16 * k) * DP * 2 + p * PLANE + dt / NT * NT * 64;
+                            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][0] + imm));
+                            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][1] + imm));
                             x[p] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
                         }
-                        if constexpr (PL == 3) {
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], w[0], o[dt], 0, 0, 0);
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[2], o[dt], 0, 0, 0);
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[1], o[dt], 0, 0, 0);
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[0], o[dt], 0, 0, 0);
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[1], o[dt], 0, 0, 0);
+#pragma unroll
+                        for (int u = 0; u < UT; ++u) {
+                            if constexpr (PL == 3) {
+                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], w[u][k][0], o[u][dt], 0, 0, 0);
+                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][2], o[u][dt], 0, 0, 0);
+                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[u][k][1], o[u][dt], 0, 0, 0);
+                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[u][k][0], o[u][dt], 0, 0, 0);
+                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][1], o[u][dt], 0, 0, 0);
+                            }
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][0], o[u][dt], 0, 0, 0);
                         }
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[0], o[dt], 0, 0, 0);
+                        if (dt % SCHED == SCHED - 1) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
         }
+        const uint32_t by = buf ? -BUF : BUF;
+#pragma unroll
+        for (int s = 0; s < NA; ++s) at_a[s] += by;
+#pragma unroll
+        for (int d = 0; d < NT; ++d) { at_t[d][0] += by; at_t[d][1] += by; }
+        at_i += buf ? -TB * 4 : TB * 4;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
 
-    if (st0 + col >= a.n_st) return;
-    const int64_t at = (int64_t)split * a.n_st + st0 + col;
-    if (MODE != TABLE || a.part_s) {
-        const float both = sum + __shfl_xor(sum, 32, 64);     // the two lanes of a row leave the kernel together
-        if (kh == 0) {
-            if constexpr (MODE != TABLE) a.part_m[at] = m;
-            a.part_s[at] = both;
+#pragma unroll
+    for (int u = 0; u < UT; ++u) {
+        const int32_t row = st0 + 32 * u + col;
+        const float both = sum[u] + __shfl_xor(sum[u], 32, 64);
+        if (row >= n_st) continue;
+        const int64_t out = (int64_t)split * n_st + row;
+        if ((MODE != TABLE || a.part_s) && kh == 0) {
+            if constexpr (MODE != TABLE) a.part_m[out] = m[u];
+            a.part_s[out] = both;
         }
-    }
-    if constexpr (MODE != LOSS) {
+        if constexpr (MODE != LOSS) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f32x4 v;
+                for (int j = 0; j < 4; ++j) {
+                    f32x4 v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = o[dt][4 * j + i];
-                *(f32x4 *)(a.part_o + at * DP + 32 * dt + 8 * j + 4 * kh) = v;
-            }
+                    for (int i = 0; i < 4; ++i) v[i] = o[u][dt][4 * j + i];
+                    *(f32x4 *)(a.part_o + out * DP + 32 * dt + 8 * j + 4 * kh) = v;
+                }
+        }
     }
 }
 
@@ -414,7 +507,7 @@ __global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ pa
 }
 
 struct LossPlan {
-    int dp, planes, nw1, splits1, rt1, splits2, rt2;
+    int dp, planes, splits1, rt1, splits2, rt2;
     bool copy_w;
     int64_t xp, wp, targets, m1, s1, o1, init, q, g, s2, o2, bytes;
 };
@@ -436,10 +529,10 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
     p.planes = dtype == MFSGD_F32 ? 3 : 1;
     const int tb = tile_rows(p.dp, p.planes);
-    p.nw1 = 4;
-    p.rt1 = (int)((n + 32 * p.nw1 - 1) / (32 * p.nw1));
+    const int rows = p.planes == 3 || (grads && p.dp > 128) ? 128 : 256;        // stationary rows a workgroup
+    p.rt1 = (int)((n + rows - 1) / rows);
     p.splits1 = parts_of((n_items + tb - 1) / tb, p.rt1, 512);
-    p.rt2 = (int)((n_items + 127) / 128);
+    p.rt2 = (int)((n_items + rows - 1) / rows);
     p.splits2 = parts_of((n + tb - 1) / tb, p.rt2, 512);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
@@ -461,8 +554,8 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
 template <int DP, int PL, int MODE>
 int launch_stream(const StreamArgs &a, hipStream_t st)
 {
-    auto kern = k_stream<DP, PL, 4, MODE>;
-    constexpr int bytes = Shape<DP, PL>::LDS;
+    auto kern = k_stream<DP, PL, MODE>;
+    constexpr int bytes = Shape<DP, PL, MODE>::LDS;
     static_assert(bytes <= 160 * 1024, "a CU's LDS");
     MF_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.splits * a.row_tiles)), dim3(256), bytes, st, a);
