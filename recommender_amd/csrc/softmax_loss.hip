@@ -41,35 +41,115 @@ constexpr float SLACK = 8.f;
 
 enum { LOSS = 0, LOSS_SUMS = 1, TABLE = 2 };   // pass 1 without / with the weighted sums, pass 2
 
+struct Rows {                           // rows as the caller has them
+    const void *p;
+    int64_t stride;
+    int32_t n, vec;                     // vec: elements a load may take
+};
+
 struct StreamArgs {
-    const __bf16 *st, *sm;              // planes of stationary / streamed rows, DP wide, zero padded
-    int64_t st_stride, st_plane, sm_stride, sm_plane;
-    int64_t n_st, n_sm;
-    const int32_t *targets;             // of the x rows (padding and ids outside the table: -1)
+    Rows st, sm;                        // stationary rows; streamed rows where they are converted on the way (CONV)
+    const __bf16 *sm_planes;            // else: planes of the streamed rows, DP wide, zero padded
+    int64_t planes_stride, plane;
+    int32_t d, n_items;
+    const int32_t *targets;             // of the x rows
     const float *bias;                  // of the items, may be NULL
     float c, inv_scale;                 // scale log2(e), 1 / scale
     int32_t splits, row_tiles;
-    float *part_m, *part_s;             // pass 1 [splits][n_st]; pass 2: part_s = sums of G for the bias
-    float *part_o;                      // [splits][n_st][DP]
+    float *part_m, *part_s;             // pass 1 [splits][rows]; pass 2: part_s = sums of G for the bias, NULL: not wanted
+    float *part_o;                      // [splits][rows][DP]; pass 2, splits == 1: NULL, the result goes to out
     const float *row_init, *row_q, *row_g;   // pass 2: -lse / scale, g (1 - p_t), g (g: the row's weight, NULL: all 1)
+    void *out;                          // pass 2: dW [n_items][d] of the rows' type, times out_f
+    float *out_b;                       // and db, times weight
+    float out_f, weight;
+    int32_t out_vec;
 };
 
-// UT: 32-row tiles of stationary rows a wave keeps.
-template <int DP, int PL, int MODE> struct Shape {
+// 8 elements of a row from column c on, zero behind column d
+template <typename T> struct Piece;
+template <> struct Piece<float> { float v[8]; };
+template <> struct Piece<__bf16> { uint32_t v[4]; };
+__device__ __forceinline__ void load_piece(const float *row, int32_t c, int32_t d, int32_t vec, Piece<float> &o)
+{
+    if (c + 8 <= d && vec >= 2) {
+        if (vec == 4) {
+            *(float4 *)(o.v) = *(const float4 *)(row + c);
+            *(float4 *)(o.v + 4) = *(const float4 *)(row + c + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) *(float2 *)(o.v + i) = *(const float2 *)(row + c + i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = row[c + i < d ? c + i : 0];
+            o.v[i] = c + i < d ? t : 0.f;
+        }
+    }
+}
+__device__ __forceinline__ void load_piece(const __bf16 *row, int32_t c, int32_t d, int32_t vec, Piece<__bf16> &o)
+{
+    if (c + 8 <= d && vec >= 2) {
+        if (vec == 8) *(uint4 *)o.v = *(const uint4 *)(row + c);
+        else if (vec == 4) {
+            *(uint2 *)o.v = *(const uint2 *)(row + c);
+            *(uint2 *)(o.v + 2) = *(const uint2 *)(row + c + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.v[i] = *(const uint32_t *)(row + c + 2 * i);
+        }
+    } else {
+        const uint16_t *bits = (const uint16_t *)row;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = bits[c + 2 * i < d ? c + 2 * i : 0], hi = bits[c + 2 * i + 1 < d ? c + 2 * i + 1 : 0];
+            o.v[i] = (c + 2 * i < d ? lo : 0) | (c + 2 * i + 1 < d ? hi << 16 : 0);
+        }
+    }
+}
+// ... as matrix operands: a bf16 piece as it is, an fp32 piece as three of which the sum is exact to 2^-24
+__device__ __forceinline__ void split_piece(const Piece<__bf16> &in, bool live, bf16x8 (&out)[1])
+{
+    const uint4 u = live ? make_uint4(in.v[0], in.v[1], in.v[2], in.v[3]) : make_uint4(0, 0, 0, 0);
+    out[0] = __builtin_bit_cast(bf16x8, u);
+}
+__device__ __forceinline__ void split_piece(const Piece<float> &in, bool live, bf16x8 (&out)[3])
+{
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = live ? in.v[i] : 0.f;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            v[2 * i] -= bf16_lo(u[i]);
+            v[2 * i + 1] -= bf16_hi(u[i]);
+        }
+        out[p] = __builtin_bit_cast(bf16x8, *(const uint4 *)u);
+    }
+}
+
 #ifndef UTX
-#define UTX (PL == 3 || (MODE != LOSS && DP > 128) ? 1 : 2)
+#define UTX (PL == 3 || CONV || (MODE != LOSS && DP > 64) ? 1 : 2)
 #endif
 #ifndef RX
-#define RX 40
+#define RX 48
 #endif
-    static constexpr int UT = UTX;
-    static constexpr int TB = (PL == 3 && DP > 32) ? 32 : 64;        // streamed rows a tile
+template <int DP, int PL, int MODE, bool CONV> struct Shape {
+    static constexpr int UT = UTX;                                   // 32-row tiles of stationary rows a wave keeps
+    static constexpr int ROWS = 128 * UT;                            // stationary rows a workgroup
+    static constexpr int NB = DP == 256 && MODE != LOSS ? (PL == 1 ? 8 : 4) : 0;     // sixteenths of a stationary row that wait in LDS
+    static constexpr int TB = ((PL == 3 || CONV) && DP > 32) || NB ? 32 : 64;      // streamed rows a tile
     static constexpr int CH = DP / 8;                                // 16-byte pieces of a row
     static constexpr int BUF = PL * TB * DP * 2;                     // bytes of a tile
-    static constexpr int LDS = 2 * BUF + 2 * TB * 16;
-    // registers: the stationary rows, the sums, the logits and what is in flight; two waves a SIMD have 256 each
-    static constexpr int REGS = UT * PL * DP / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + RX;
-    static constexpr int WAVES = REGS <= 256 ? 2 : 1;
+    static constexpr int LDS = 2 * BUF + 2 * TB * 16 + NB * PL * 4096;
+    static constexpr int HOLD = CONV ? TB * CH / 256 : 0;            // pieces a thread holds on their way to LDS
+    // registers: the stationary rows, the sums, the logits and what is in flight
+    static constexpr int REGS = UT * PL * (DP - 16 * NB) / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + HOLD * (PL == 3 ? 8 : 4) + (CONV ? 20 : 0) + RX;
+    static constexpr int WAVES = REGS <= 120 ? 4 : REGS <= 156 ? 3 : REGS <= 256 ? 2 : 1;        // a SIMD
+    static constexpr int GROUPS = WAVES < 160 * 1024 / LDS ? WAVES : 160 * 1024 / LDS;           // workgroups a CU
 };
 
 // Piece c of row r lies at piece c ^ swizzle(r).  The logits' operand takes one piece of 16 consecutive rows at a time, the
@@ -81,15 +161,17 @@ template <int CH> __device__ __forceinline__ int swizzle(int r)
     else return (r & 2) | ((r >> 2) & 1);
 }
 
-template <int DP, int PL, int MODE>
-__global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(const StreamArgs a)
+template <typename T, int DP, int MODE, bool CONV>
+__global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>::WAVES)) void k_stream(const StreamArgs a)
 {
-    using S = Shape<DP, PL, MODE>;
+    constexpr int PL = sizeof(T) == 4 ? 3 : 1;
+    using S = Shape<DP, PL, MODE, CONV>;
     constexpr int UT = S::UT, TB = S::TB, CH = S::CH, BUF = S::BUF, KS = DP / 16, DT = DP / 32, PLANE = TB * DP * 2;
-    constexpr int Q = BUF / 4096;
-#ifndef SCHED
-#define SCHED 4
+    constexpr int Q = BUF / 4096, HOLD = S::HOLD;
+#ifndef GAX
+#define GAX (PL == 3 ? 1 : 2)
 #endif
+    constexpr int GA = GAX;
     static_assert(BUF % 4096 == 0, "a tile is a whole number of 1 KB pieces per wave");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *l_init = (float *)(lds + 2 * BUF);           // [2][TB]
@@ -107,52 +189,77 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
         split = blockIdx.x / a.row_tiles;
         rt = blockIdx.x % a.row_tiles;
     }
-    const int32_t n_st = (int32_t)a.n_st, n_sm = (int32_t)a.n_sm;            // both below 2^29
+    const int32_t n_st = a.st.n, n_sm = a.sm.n;
     const int32_t st0 = (rt * 4 + wave) * (32 * UT);
     const int32_t tiles = (n_sm + TB - 1) / TB;
     const int32_t t0 = (int32_t)((int64_t)tiles * split / a.splits), t1 = (int32_t)((int64_t)tiles * (split + 1) / a.splits);
 
-    bf16x8 b[UT][PL][KS];
+    constexpr int NB = S::NB, KR = KS - NB;
+    bf16x8 b[UT][PL][KR];
+    LDS_AS char *l_b = (LDS_AS char *)lds + 2 * BUF + 2 * TB * 16 + (wave * NB * PL * 64 + lane) * 16;
     int32_t target[UT];
     float b2[UT];
 #pragma unroll
     for (int u = 0; u < UT; ++u) {
         const int32_t row = std::min(st0 + 32 * u + col, n_st - 1);
-        target[u] = MODE == TABLE ? -1 : a.targets[row];
+        target[u] = MODE == TABLE ? 0 : a.targets[row];
+        const bool live = MODE == TABLE || (uint32_t)target[u] < (uint32_t)a.n_items;        // padding is not looked at
         b2[u] = (MODE == TABLE && a.bias) ? a.bias[row] * LOG2E : 0.f;
 #pragma unroll
-        for (int p = 0; p < PL; ++p)
+        for (int s = 0; s < KS; ++s) {
+            Piece<T> raw;
+            bf16x8 v[PL];
+            load_piece((const T *)a.st.p + row * a.st.stride, 16 * s + 8 * kh, a.d, a.st.vec, raw);
+            split_piece(raw, live, v);
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                b[u][p][s] = *(const bf16x8 *)(a.st + p * a.st_plane + row * a.st_stride + 16 * s + 8 * kh);
+            for (int p = 0; p < PL; ++p) {
+                if (s < KR) b[u][p][s] = v[p];
+                else *(LDS_AS bf16x8 *)(l_b + ((s - KR) * PL + p) * 1024) = v[p];       // read by the same lane only
+            }
+        }
     }
 
     // A tile goes straight from memory to LDS, 1 KB a wave and instruction; its place is the lane's, so the swizzle is in
-    // which piece a lane asks for.
+    // which piece a lane asks for.  Where few workgroups read the streamed rows (CONV) they take them as they are and
+    // convert them on the way, through registers.
     constexpr int STEP = 256 / CH;                      // rows an instruction of the whole workgroup covers
     constexpr bool EVEN = 256 % CH == 0;
     int32_t from[2];                                    // a lane's offset in the rows of even and odd steps
 #pragma unroll
-    for (int v = 0; v < 2; ++v) from[v] = (tid / CH) * (int32_t)a.sm_stride + ((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 8;
+    for (int v = 0; v < 2; ++v) from[v] = (tid / CH) * (int32_t)a.planes_stride + ((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 8;
+    Piece<T> hold[HOLD ? HOLD : 1];
+    uint32_t held = 0;                                  // bit q: row of piece q takes part
     auto stage = [&](int32_t t, int buf) {
-        const __bf16 *base = a.sm + (int64_t)t * TB * a.sm_stride;
         const int32_t last = std::min(TB, n_sm - t * TB) - 1;
-        if (EVEN && last == TB - 1) {
+        if constexpr (CONV) {
+            held = 0;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                constexpr int PER = Q / PL;
-                const __bf16 *rows = base + (q / PER) * a.sm_plane + (q % PER) * STEP * a.sm_stride;
-                __builtin_amdgcn_global_load_lds((const GLB_AS void *)(rows + from[q % PER % 2]),
-                                                 (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < HOLD; ++q) {
+                const int slot = q * 256 + tid, r = slot / CH, c = (slot % CH) ^ swizzle<CH>(slot / CH);
+                const int32_t row = t * TB + std::min(r, last);
+                const bool live = MODE != TABLE || (uint32_t)a.targets[row] < (uint32_t)a.n_items;
+                held |= (uint32_t)live << q;
+                load_piece((const T *)a.sm.p + row * a.sm.stride, c * 8, a.d, a.sm.vec, hold[q]);
             }
-        } else {                                        // rows behind the last one are the last one, masked below
+        } else {
+            const __bf16 *base = a.sm_planes + (int64_t)t * TB * a.planes_stride;
+            if (EVEN && last == TB - 1) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    constexpr int PER = Q / PL;
+                    const __bf16 *rows = base + (q / PER) * a.plane + (q % PER) * STEP * a.planes_stride;
+                    __builtin_amdgcn_global_load_lds((const GLB_AS void *)(rows + from[q % PER % 2]),
+                                                     (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {                                    // rows behind the last one are the last one, masked below
 #pragma unroll 1
-            for (int q = 0; q < Q; ++q) {
-                const int slot = q * 256 + tid;
-                const int p = slot / (TB * CH), r = slot / CH % TB, c = (slot % CH) ^ swizzle<CH>(slot / CH % TB);
-                __builtin_amdgcn_global_load_lds((const GLB_AS void *)(base + p * a.sm_plane + std::min(r, last) * a.sm_stride + c * 8),
-                                                 (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
+                for (int q = 0; q < Q; ++q) {
+                    const int slot = q * 256 + tid;
+                    const int p = slot / (TB * CH), r = slot / CH % TB, c = (slot % CH) ^ swizzle<CH>(slot / CH % TB);
+                    __builtin_amdgcn_global_load_lds((const GLB_AS void *)(base + p * a.plane + std::min(r, last) * a.planes_stride + c * 8),
+                                                     (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
+                }
             }
         }
         if (tid < TB) {
@@ -166,6 +273,19 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
             } else
                 l_init[buf * TB + tid] = in ? (a.bias ? a.bias[row] * a.inv_scale : 0.f) : -INFINITY;
         }
+    };
+    auto commit = [&](int buf) {                        // what stage() began is in LDS afterwards
+        if constexpr (CONV) {
+#pragma unroll
+            for (int q = 0; q < HOLD; ++q) {
+                bf16x8 v[PL];
+                split_piece(hold[q], (held >> q) & 1, v);
+#pragma unroll
+                for (int p = 0; p < PL; ++p) *(bf16x8 *)(lds + buf * BUF + p * PLANE + (q * 256 + tid) * 16) = v[p];
+            }
+        } else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     };
 
     f32x16 o[UT][MODE == LOSS ? 1 : DT];
@@ -192,9 +312,24 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
         for (int h = 0; h < 2; ++h)
             at_t[d][h] = (tr + 8 * h) * DP * 2 + ((4 * d + 2 * half + ((i16 & 3) >> 1)) ^ swizzle<CH>(tr + 8 * h)) * 16 + (i16 & 1) * 8;
 
+    // operands: 16 columns of 32 streamed rows for the logits, 32 columns of 16 streamed rows, transposed, for the sums
+    auto load_a = [&](int sub, int s, bf16x8 (&x)[PL]) {
+#pragma unroll
+        for (int p = 0; p < PL; ++p) x[p] = *(const LDS_AS bf16x8 *)(l3 + at_a[s % NA] + (sub * 32 * DP * 2 + p * PLANE + s / NA * NA * 32));
+    };
+    auto load_t = [&](int sub, int n, bf16x8 (&x)[PL]) {
+        const int k = n / DT, dt = n % DT;
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+            const int imm = (sub * 32 + 16 * k) * DP * 2 + p * PLANE + dt / NT * NT * 64;
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][0] + imm));
+            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][1] + imm));
+            x[p] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+
     if (t0 < t1) stage(t0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    commit(0);
     for (int32_t t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1;
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
@@ -210,23 +345,39 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
             }
 #pragma unroll
             for (int u = 1; u < UT; ++u) acc[u] = acc[0];
+            // operands are read one group ahead of the products that take them
+            bf16x8 x[2][GA][PL];
+#pragma unroll
+            for (int q = 0; q < GA; ++q) load_a(sub, q, x[0][q]);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                bf16x8 x[PL];
+                if (s % GA == 0) {
+                    if (s) __builtin_amdgcn_sched_barrier(0);
+                    if (s + GA < KS) {
 #pragma unroll
-                for (int p = 0; p < PL; ++p) x[p] = *(const LDS_AS bf16x8 *)(l3 + at_a[s % NA] + (sub * 32 * DP * 2 + p * PLANE + s / NA * NA * 32));
+                        for (int q = 0; q < GA; ++q) load_a(sub, s + GA + q, x[(s / GA + 1) & 1][q]);
+                    }
+                }
+                const bf16x8 (&y)[PL] = x[(s / GA) & 1][s % GA];
 #pragma unroll
                 for (int u = 0; u < UT; ++u) {
+                    bf16x8 z[PL];
+#pragma unroll
+                    for (int p = 0; p < PL; ++p) z[p] = s < KR ? b[u][p][s < KR ? s : 0] : *(const LDS_AS bf16x8 *)(l_b + ((s - KR) * PL + p) * 1024);
                     if constexpr (PL == 3) {
-                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], b[u][0][s], acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][2][s], acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[u][1][s], acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], b[u][0][s], acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][1][s], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[2], z[0], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], z[2], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], z[1], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], z[0], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], z[1], acc[u], 0, 0, 0);
                     }
-                    acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], b[u][0][s], acc[u], 0, 0, 0);
+                    acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], z[0], acc[u], 0, 0, 0);
                 }
-                if (s % SCHED == SCHED - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (MODE != LOSS) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int q = 0; q < GA; ++q) load_t(sub, q, x[0][q]);
             }
             bf16x8 w[UT][2][PL];       // the exponentials as operands: j 0..7 and 8..15
             uint32_t hits = 0, at = 0;
@@ -322,29 +473,26 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
             if constexpr (MODE != LOSS) {
                 // o[u][dt][j] += sum over the 32 streamed rows of their column 32 dt + 8 (j / 4) + 4 kh + j % 4 times e
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int n = 0; n < 2 * DT; ++n) {
+                    if (n % GA == 0) {
+                        if (n) __builtin_amdgcn_sched_barrier(0);
+                        if (n + GA < 2 * DT) {
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        bf16x8 x[PL];
-#pragma unroll
-                        for (int p = 0; p < PL; ++p) {
-                            const int imm = (sub * 32 + 16 * k) * DP * 2 + p * PLANE + dt / NT * NT * 64;
-                            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][0] + imm));
-                            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][1] + imm));
-                            x[p] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+                            for (int q = 0; q < GA; ++q) load_t(sub, n + GA + q, x[(n / GA + 1) & 1][q]);
                         }
+                    }
+                    const bf16x8 (&y)[PL] = x[(n / GA) & 1][n % GA];
+                    const int k = n / DT, dt = n % DT;
 #pragma unroll
-                        for (int u = 0; u < UT; ++u) {
-                            if constexpr (PL == 3) {
-                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], w[u][k][0], o[u][dt], 0, 0, 0);
-                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][2], o[u][dt], 0, 0, 0);
-                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[u][k][1], o[u][dt], 0, 0, 0);
-                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], w[u][k][0], o[u][dt], 0, 0, 0);
-                                o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][1], o[u][dt], 0, 0, 0);
-                            }
-                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], w[u][k][0], o[u][dt], 0, 0, 0);
+                    for (int u = 0; u < UT; ++u) {
+                        if constexpr (PL == 3) {
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[2], w[u][k][0], o[u][dt], 0, 0, 0);
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], w[u][k][2], o[u][dt], 0, 0, 0);
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], w[u][k][1], o[u][dt], 0, 0, 0);
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], w[u][k][0], o[u][dt], 0, 0, 0);
+                            o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], w[u][k][1], o[u][dt], 0, 0, 0);
                         }
-                        if (dt % SCHED == SCHED - 1) __builtin_amdgcn_sched_barrier(0);
+                        o[u][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], w[u][k][0], o[u][dt], 0, 0, 0);
                     }
                 }
             }
@@ -355,8 +503,7 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
 #pragma unroll
         for (int d = 0; d < NT; ++d) { at_t[d][0] += by; at_t[d][1] += by; }
         at_i += buf ? -TB * 4 : TB * 4;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        commit(buf ^ 1);
     }
 
 #pragma unroll
@@ -365,55 +512,59 @@ __global__ __launch_bounds__(256, (Shape<DP, PL, MODE>::WAVES)) void k_stream(co
         const float both = sum[u] + __shfl_xor(sum[u], 32, 64);
         if (row >= n_st) continue;
         const int64_t out = (int64_t)split * n_st + row;
-        if ((MODE != TABLE || a.part_s) && kh == 0) {
-            if constexpr (MODE != TABLE) a.part_m[out] = m[u];
-            a.part_s[out] = both;
+        if (kh == 0) {
+            if constexpr (MODE != TABLE) {
+                a.part_m[out] = m[u];
+                a.part_s[out] = both;
+            } else if (a.part_s) {
+                if (a.part_o) a.part_s[out] = both;
+                else a.out_b[row] = both * a.weight;
+            }
         }
         if constexpr (MODE != LOSS) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    f32x4 v;
+                    const int c = 32 * dt + 8 * j + 4 * kh;
+                    if (MODE == LOSS_SUMS || a.part_o) {
+                        f32x4 v;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = o[u][dt][4 * j + i];
-                    *(f32x4 *)(a.part_o + out * DP + 32 * dt + 8 * j + 4 * kh) = v;
+                        for (int i = 0; i < 4; ++i) v[i] = o[u][dt][4 * j + i];
+                        *(f32x4 *)(a.part_o + out * DP + c) = v;
+                    } else if (c < a.d) {
+                        T *dst = (T *)a.out + (int64_t)row * a.d + c;
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = o[u][dt][4 * j + i] * a.out_f;
+                        if (a.out_vec >= 4) store_vec<4>(dst, v);
+                        else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) if (c + i < a.d) store_f32(dst + i, v[i]);
+                        }
+                    }
                 }
         }
     }
 }
 
-// rows -> planes of bf16, DP wide, columns from d on zero; with targets: the rows that take no part are zero, their target -1
+// rows -> planes of bf16, dp wide, columns from d on zero; with targets: the rows that take no part are zero
 template <typename T, int PL>
-__global__ __launch_bounds__(256) void k_planes(const T *__restrict__ src, int64_t stride, int64_t n, int32_t d, int32_t dp,
-                                                const int32_t *__restrict__ targets, int64_t n_items, __bf16 *__restrict__ dst,
-                                                int32_t *__restrict__ targets_out)
+__global__ __launch_bounds__(256) void k_planes(const Rows src, int32_t d, int32_t dp, const int32_t *__restrict__ targets, int32_t n_items,
+                                                __bf16 *__restrict__ dst)
 {
     const int32_t per = dp / 8;
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p >= n * per) return;
+    if (p >= (int64_t)src.n * per) return;
     const int64_t r = p / per;
     const int32_t c = (int32_t)(p - r * per) * 8;
-    bool in = true;
-    if (targets) {
-        const int32_t t = targets[r];
-        in = (uint32_t)t < (uint64_t)n_items;
-        if (c == 0) targets_out[r] = in ? t : -1;
-    }
-    float v[8];
+    const bool live = !targets || (uint32_t)targets[r] < (uint32_t)n_items;
+    Piece<T> raw;
+    bf16x8 v[PL];
+    load_piece((const T *)src.p + r * src.stride, c, d, src.vec, raw);
+    split_piece(raw, live, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = in && c + i < d ? load_f32(src + r * stride + c + i) : 0.f;
-#pragma unroll
-    for (int q = 0; q < PL; ++q) {
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            u[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-            v[2 * i] -= bf16_lo(u[i]);
-            v[2 * i + 1] -= bf16_hi(u[i]);
-        }
-        *(uint4 *)(dst + (int64_t)q * n * dp + r * dp + c) = *(const uint4 *)u;
-    }
+    for (int q = 0; q < PL; ++q) *(bf16x8 *)(dst + (int64_t)q * src.n * dp + r * dp + c) = v[q];
 }
 
 struct JoinArgs {
@@ -476,14 +627,29 @@ __global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__r
         a.row_q[r] = q * g;
         if (a.row_g) a.row_g[r] = none ? 0.f : g;
     }
+    // four columns a lane, the parts dealt to 64 / lanes groups of lanes
     const float f = g * a.weight * a.scale;
-    for (int c = lane; c < a.d; c += 64) {
-        float v = 0.f;
-        for (int s = 0; s < a.splits; ++s)
-            v += a.part_o[((int64_t)s * a.n + r) * a.dp + c] * __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);
-        const float out = none ? 0.f : f * (v / all - q * load_f32(w + (int64_t)t * a.w_stride + c));
-        store_f32(dx + r * a.d + c, out);
+    const int lanes = a.dp > 128 ? 64 : a.dp > 64 ? 32 : a.dp > 32 ? 16 : 8;        // dp = 192: 48 of 64 busy
+    const int c = lane % lanes * 4, step = 64 / lanes;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.dp) {
+#pragma unroll 4
+        for (int s = lane / lanes; s < a.splits; s += step) {
+            const float w2 = __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);
+            const f32x4 p = *(const f32x4 *)(a.part_o + ((int64_t)s * a.n + r) * a.dp + c);
+            v += p * w2;
+        }
     }
+    for (int k = lanes; k < 64; k <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], k, 64);
+    if (lane < lanes)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < a.d) {
+                const float out = none ? 0.f : f * (v[i] / all - q * load_f32(w + (int64_t)t * a.w_stride + c + i));
+                store_f32(dx + r * a.d + c + i, out);
+            }
 }
 
 // the parts of the rows' axis of pass 2, summed in order: dW and db
@@ -506,21 +672,44 @@ __global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ pa
     }
 }
 
+// Workgroups of a pass at once on the chip, stationary rows a workgroup and streamed rows a tile, by the kernel's shape
+struct PassShape { int groups, rows, tile; };
+template <int PL, int MODE, bool CONV>
+PassShape pass_shape_d(int dp)
+{
+#define MF_SHAPE(DP_) case DP_: { using S = Shape<DP_, PL, MODE, CONV>; return {256 * S::GROUPS, S::ROWS, S::TB}; }
+    switch (dp) { MF_SHAPE(32) MF_SHAPE(64) MF_SHAPE(128) MF_SHAPE(192) default: MF_SHAPE(256) }
+#undef MF_SHAPE
+}
+template <int PL>
+PassShape pass_shape(int dp, int mode, bool conv)
+{
+    if (mode == LOSS) return conv ? pass_shape_d<PL, LOSS, true>(dp) : pass_shape_d<PL, LOSS, false>(dp);
+    if (mode == LOSS_SUMS) return conv ? pass_shape_d<PL, LOSS_SUMS, true>(dp) : pass_shape_d<PL, LOSS_SUMS, false>(dp);
+    return conv ? pass_shape_d<PL, TABLE, true>(dp) : pass_shape_d<PL, TABLE, false>(dp);
+}
+
+// Parts the streamed axis is cut into.  A workgroup's time counts in tiles (HEAD more for its start and end), the parts' sums
+// are written and read again (PART tiles a part, if a workgroup's share of memory were all it waited for): the number of
+// parts with the least rounds x (tiles + HEAD) + parts x PART.
+int parts_of(int64_t n_sm, int64_t row_tiles, const PassShape &s, double head, double part)
+{
+    const int64_t tiles = (n_sm + s.tile - 1) / s.tile;
+    int best = 1;
+    double least = 1e300;
+    for (int k = 1; k <= 1024 && k <= tiles; k += k < 8 ? 1 : 8 - k % 8) {
+        const int64_t rounds = (row_tiles * k + s.groups - 1) / s.groups;
+        const double cost = rounds * ((tiles + k - 1) / k + head) + (k > 1 ? k * part * rounds * s.groups / (row_tiles * k) : 0.0);
+        if (cost < least * 0.999) { least = cost; best = k; }
+    }
+    return best;
+}
+
 struct LossPlan {
     int dp, planes, splits1, rt1, splits2, rt2;
-    bool copy_w;
-    int64_t xp, wp, targets, m1, s1, o1, init, q, g, s2, o2, bytes;
+    bool conv;
+    int64_t xp, wp, m1, s1, o1, init, q, g, s2, o2, bytes;
 };
-
-int tile_rows(int dp, int planes) { return planes == 3 && dp > 32 ? 32 : 64; }
-
-// Parts an axis of `tiles` tiles is cut into so that `row_tiles` workgroups a part give the chip two per CU
-int parts_of(int64_t tiles, int64_t row_tiles, int64_t want)
-{
-    int64_t s = std::min(tiles, (want + row_tiles - 1) / row_tiles);
-    if (s > 8) s = s / 8 * 8;
-    return (int)std::max<int64_t>(1, s);
-}
 
 LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool grads)
 {
@@ -528,34 +717,41 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     n = std::max<int64_t>(n, 1);
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
     p.planes = dtype == MFSGD_F32 ? 3 : 1;
-    const int tb = tile_rows(p.dp, p.planes);
-    const int rows = p.planes == 3 || (grads && p.dp > 128) ? 128 : 256;        // stationary rows a workgroup
-    p.rt1 = (int)((n + rows - 1) / rows);
-    p.splits1 = parts_of((n_items + tb - 1) / tb, p.rt1, 512);
-    p.rt2 = (int)((n_items + rows - 1) / rows);
-    p.splits2 = parts_of((n + tb - 1) / tb, p.rt2, 512);
+    const int mode1 = grads ? LOSS_SUMS : LOSS;
+    auto shape = [&](int mode, bool conv) { return p.planes == 3 ? pass_shape<3>(p.dp, mode, conv) : pass_shape<1>(p.dp, mode, conv); };
+    // with one row tile the items are read once either way: converting them on the way saves a launch and a round trip
+    // (fp32 rows of 256 with gradients leave no registers for it)
+    p.conv = n <= shape(mode1, true).rows && !(p.planes == 3 && p.dp == 256 && grads);
+    const PassShape s1 = shape(mode1, p.conv), s2 = shape(TABLE, p.conv);
+    p.rt1 = (int)((n + s1.rows - 1) / s1.rows);
+    p.splits1 = parts_of(n_items, p.rt1, s1, 2.0, 0.5);
+    p.rt2 = (int)((n_items + s2.rows - 1) / s2.rows);
+    p.splits2 = parts_of(n, p.rt2, s2, 2.0, 1.0);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
-    p.xp = take((int64_t)p.planes * n * p.dp * 2);
-    p.wp = take((int64_t)p.planes * n_items * p.dp * 2);       // not used where the table's rows are operands as they are
-    p.targets = take(n * 4);
+    if (!p.conv) {
+        if (grads) p.xp = take((int64_t)p.planes * n * p.dp * 2);
+        p.wp = take((int64_t)p.planes * n_items * p.dp * 2);       // not used where the table's rows are operands as they are
+    }
     p.m1 = take((int64_t)p.splits1 * n * 4);
     p.s1 = take((int64_t)p.splits1 * n * 4);
     if (grads) {
         p.o1 = take((int64_t)p.splits1 * n * p.dp * 4);
         p.init = take(n * 4); p.q = take(n * 4); p.g = take(n * 4);
-        p.s2 = take((int64_t)p.splits2 * n_items * 4);
-        p.o2 = take((int64_t)p.splits2 * n_items * p.dp * 4);
+        if (p.splits2 > 1) {
+            p.s2 = take((int64_t)p.splits2 * n_items * 4);
+            p.o2 = take((int64_t)p.splits2 * n_items * p.dp * 4);
+        }
     }
     p.bytes = std::max<int64_t>(at, 256);
     return p;
 }
 
-template <int DP, int PL, int MODE>
+template <typename T, int DP, int MODE, bool CONV>
 int launch_stream(const StreamArgs &a, hipStream_t st)
 {
-    auto kern = k_stream<DP, PL, MODE>;
-    constexpr int bytes = Shape<DP, PL, MODE>::LDS;
+    auto kern = k_stream<T, DP, MODE, CONV>;
+    constexpr int bytes = Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>::LDS;
     static_assert(bytes <= 160 * 1024, "a CU's LDS");
     MF_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.splits * a.row_tiles)), dim3(256), bytes, st, a);
@@ -563,47 +759,50 @@ int launch_stream(const StreamArgs &a, hipStream_t st)
     return MFSGD_OK;
 }
 
-template <int PL, int MODE>
-int launch_stream_d(int dp, const StreamArgs &a, hipStream_t st)
+template <typename T, int MODE>
+int launch_stream_d(int dp, bool conv, const StreamArgs &a, hipStream_t st)
 {
-    switch (dp) {
-        case 32: return launch_stream<32, PL, MODE>(a, st);
-        case 64: return launch_stream<64, PL, MODE>(a, st);
-        case 128: return launch_stream<128, PL, MODE>(a, st);
-        case 192: return launch_stream<192, PL, MODE>(a, st);
-        default: return launch_stream<256, PL, MODE>(a, st);
-    }
+#define MF_STREAM(DP_) case DP_: return conv ? launch_stream<T, DP_, MODE, true>(a, st) : launch_stream<T, DP_, MODE, false>(a, st);
+    switch (dp) { MF_STREAM(32) MF_STREAM(64) MF_STREAM(128) MF_STREAM(192) }
+#undef MF_STREAM
+    if constexpr (sizeof(T) == 2 || MODE == LOSS) if (conv) return launch_stream<T, 256, MODE, true>(a, st);
+    return launch_stream<T, 256, MODE, false>(a, st);
 }
 
-template <typename T, int PL>
+template <typename T>
 int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *targets, const float *bias, const float *weights, float weight,
               int64_t n, int64_t n_items, int32_t d, float scale, float *loss, float *lse, T *dx, T *dw, float *db, bool grads, char *ws,
               hipStream_t st)
 {
+    constexpr int PL = sizeof(T) == 4 ? 3 : 1;
     const LossPlan p = loss_plan(n, n_items, d, PL == 3 ? MFSGD_F32 : MFSGD_BF16, grads);
-    // a bf16 table whose rows are DP wide and start at multiples of 16 bytes is the operand as it is
-    const bool as_is = PL == 1 && d == p.dp && ws_ % 8 == 0 && (uintptr_t)w % 16 == 0;
+    const Rows xr = {x, xs, (int32_t)n, vec_elems(sizeof(T), 16, xs, xs, x, x)};
+    const Rows wr = {w, ws_, (int32_t)n_items, vec_elems(sizeof(T), 16, ws_, ws_, w, w)};
+    // a bf16 table whose rows are dp wide and start at multiples of 16 bytes is the operand as it is
+    const bool as_is = PL == 1 && d == p.dp && wr.vec == 8 && ws_ < (1 << 20);
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
-    int32_t *tg = (int32_t *)(ws + p.targets);
-    auto blocks = [&](int64_t rows) { return dim3((unsigned)((rows * (p.dp / 8) + 255) / 256)); };
-    hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, x, xs, n, d, p.dp, targets, n_items, xp, tg);
-    if (!as_is)
-        hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, w, ws_, n_items, d, p.dp, (const int32_t *)nullptr, n_items, wp,
-                           (int32_t *)nullptr);
-    MF_LAUNCH_CHECK();
-    const __bf16 *items = as_is ? (const __bf16 *)w : wp;
-    const int64_t items_stride = as_is ? ws_ : p.dp, items_plane = n_items * p.dp;
+    if (!p.conv) {
+        auto blocks = [&](int64_t rows) { return dim3((unsigned)((rows * (p.dp / 8) + 255) / 256)); };
+        if (grads) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, xr, d, p.dp, targets, (int32_t)n_items, xp);
+        if (!as_is) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, wr, d, p.dp, (const int32_t *)nullptr, 0, wp);
+        MF_LAUNCH_CHECK();
+    }
 
     StreamArgs a = {};
-    a.targets = tg;
+    a.d = d;
+    a.n_items = (int32_t)n_items;
+    a.targets = targets;
     a.bias = bias;
     a.c = scale * LOG2E;
     a.inv_scale = 1.f / scale;
-    a.st = xp; a.st_stride = p.dp; a.st_plane = n * p.dp; a.n_st = n;
-    a.sm = items; a.sm_stride = items_stride; a.sm_plane = items_plane; a.n_sm = n_items;
+    a.st = xr;
+    a.sm = wr;
+    a.sm_planes = as_is ? (const __bf16 *)w : wp;
+    a.planes_stride = as_is ? ws_ : p.dp;
+    a.plane = n_items * p.dp;
     a.splits = p.splits1; a.row_tiles = p.rt1;
     a.part_m = (float *)(ws + p.m1); a.part_s = (float *)(ws + p.s1); a.part_o = (float *)(ws + p.o1);
-    if (const int rc = grads ? launch_stream_d<PL, LOSS_SUMS>(p.dp, a, st) : launch_stream_d<PL, LOSS>(p.dp, a, st)) return rc;
+    if (const int rc = grads ? launch_stream_d<T, LOSS_SUMS>(p.dp, p.conv, a, st) : launch_stream_d<T, LOSS>(p.dp, p.conv, a, st)) return rc;
 
     JoinArgs j = {};
     j.n = n; j.n_items = n_items; j.x_stride = xs; j.w_stride = ws_; j.d = d; j.dp = p.dp; j.splits = p.splits1;
@@ -617,15 +816,24 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     MF_LAUNCH_CHECK();
     if (!grads) return MFSGD_OK;
 
-    a.st = items; a.st_stride = items_stride; a.st_plane = items_plane; a.n_st = n_items;
-    a.sm = xp; a.sm_stride = p.dp; a.sm_plane = n * p.dp; a.n_sm = n;
+    a.st = wr;
+    a.sm = xr;
+    a.sm_planes = xp;
+    a.planes_stride = p.dp;
+    a.plane = n * p.dp;
     a.splits = p.splits2; a.row_tiles = p.rt2;
-    a.part_m = nullptr; a.part_s = db ? (float *)(ws + p.s2) : nullptr; a.part_o = (float *)(ws + p.o2);
+    a.part_m = nullptr;
+    a.part_s = db ? (float *)(ws + p.s2) : nullptr;
+    a.part_o = p.splits2 > 1 ? (float *)(ws + p.o2) : nullptr;
     a.row_init = j.row_init; a.row_q = j.row_q; a.row_g = j.row_g;
-    if (const int rc = launch_stream_d<PL, TABLE>(p.dp, a, st)) return rc;
-    hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * d + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items, d,
-                       p.dp, scale * weight, weight, dw, db);
-    MF_LAUNCH_CHECK();
+    a.out = dw; a.out_b = db; a.out_f = scale * weight; a.weight = weight;
+    a.out_vec = vec_elems(sizeof(T), d, d, d, dw, dw);
+    if (const int rc = launch_stream_d<T, TABLE>(p.dp, p.conv, a, st)) return rc;
+    if (p.splits2 > 1) {
+        hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * d + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,
+                           d, p.dp, scale * weight, weight, dw, db);
+        MF_LAUNCH_CHECK();
+    }
     return MFSGD_OK;
 }
 
@@ -668,9 +876,9 @@ int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, i
                                   workspace_bytes, false)) return rc;
     if (n == 0) return MFSGD_OK;
     if (dtype == MFSGD_F32)
-        return loss_impl<float, 3>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
+        return loss_impl<float>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
                                    loss, lse, nullptr, nullptr, nullptr, false, (char *)workspace, as_stream(stream));
-    return loss_impl<__bf16, 1>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
+    return loss_impl<__bf16>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, nullptr, 1.f, n, n_items, d, scale,
                                 loss, lse, nullptr, nullptr, nullptr, false, (char *)workspace, as_stream(stream));
 }
 
@@ -692,9 +900,9 @@ int mfsgd_hip_softmax_loss_grads(const void *x, int64_t x_stride, const void *ta
         return MFSGD_OK;
     }
     if (dtype == MFSGD_F32)
-        return loss_impl<float, 3>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
+        return loss_impl<float>((const float *)x, x_stride, (const float *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
                                    scale, loss, lse, (float *)dx, (float *)dtable, dbias, true, (char *)workspace, st);
-    return loss_impl<__bf16, 1>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
+    return loss_impl<__bf16>((const __bf16 *)x, x_stride, (const __bf16 *)table, table_stride, targets, bias, weights, weight, n, n_items, d,
                                 scale, loss, lse, (__bf16 *)dx, (__bf16 *)dtable, dbias, true, (char *)workspace, st);
 }
 
