@@ -12,27 +12,33 @@
 namespace {
 
 // ------------------------------------------------------------------ lookup
-// A thread moves V elements (one access); the V-element pieces of the output are numbered through.
+// A thread moves PIECES pieces of V elements (one access each), all of them asked for before the first one is used; the pieces
+// of the output are numbered through.
+constexpr int PIECES = 4;
 template <typename T, int V>
-__global__ __launch_bounds__(256) void k_embedding(const T *__restrict__ table, int64_t stride, int64_t n_rows, int32_t d,
-                                                   const int32_t *__restrict__ ids, int64_t n, float scale, T *__restrict__ out)
+__global__ __launch_bounds__(256) void k_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d,
+                                                   const int32_t *__restrict__ ids, int64_t n, float scale, T *out)
 {
+    constexpr int U = PIECES;
     const int32_t per = d / V;
-    const int64_t total = n * per;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < total; p += (int64_t)gridDim.x * 256) {
-        const int64_t t = p / per;
-        const int32_t c = (int32_t)(p - t * per) * V;
-        const int32_t id = ids[t];
-        float v[V];
-        if (id >= 0 && id < n_rows) {
-            load_vec<V>(table + (int64_t)id * stride + c, v);
+    const int64_t p0 = (int64_t)blockIdx.x * (256 * U), t0 = p0 / per;          // the same for all threads
+    const int32_t skip = (int32_t)(p0 - t0 * per);
+    int32_t id[U], c[U];
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] *= scale;
-        } else {
+    for (int u = 0; u < U; ++u) {
+        const uint32_t x = skip + u * 256 + threadIdx.x, row = x / (uint32_t)per;
+        c[u] = (int32_t)(x - row * per) * V;
+        id[u] = ids[std::min<int64_t>(t0 + row, n - 1)];
+    }
+    float v[U][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = id < 0 ? 0.f : NAN;
-        }
-        store_vec<V>(out + p * V, v);
+    for (int u = 0; u < U; ++u) load_vec<V>(table + (id[u] >= 0 && id[u] < n_rows ? id[u] * stride + c[u] : 0), v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t p = p0 + u * 256 + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[u][i] = id[u] < 0 ? 0.f : id[u] < n_rows ? v[u][i] * scale : NAN;
+        if (p < n * per) store_vec<V>(out + p * V, v[u]);
     }
 }
 
@@ -40,8 +46,9 @@ template <typename T>
 int launch_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d, const int32_t *ids, int64_t n, float scale,
                      T *out, hipStream_t st)
 {
+    if (n_rows == 0) { table = out; stride = 0; }       // nothing is taken from it, but the first piece is always asked for
     const int v = vec_elems(sizeof(T), d, stride, d, table, out);
-    const unsigned grid = (unsigned)std::min<int64_t>((n * (d / v) + 255) / 256, 1 << 20);
+    const unsigned grid = (unsigned)((n * (d / v) + 256 * PIECES - 1) / (256 * PIECES));
 #define MF_EMB(V_) hipLaunchKernelGGL((k_embedding<T, V_>), dim3(grid), dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, out)
     if constexpr (sizeof(T) == 2) {
         if (v == 8) { MF_EMB(8); MF_LAUNCH_CHECK(); return MFSGD_OK; }
@@ -61,43 +68,47 @@ __device__ __forceinline__ uint32_t sort_key(int32_t id, int64_t n_rows)
     return (uint32_t)id < (uint64_t)n_rows ? (uint32_t)id : (uint32_t)n_rows;
 }
 
-// Small batches: the rank of position t is the number of smaller keys plus the number of equal keys in front of it.  A wave
-// ranks 64 positions against all keys, held in LDS; one launch, no passes.
+// Small batches: the rank of position t is the number of smaller keys plus the number of equal keys in front of it.  16 lanes
+// rank one position, a sixteenth of the keys each, read from LDS four at a time; one launch, no passes.
 constexpr int RANK_MAX = 4096;
-__global__ __launch_bounds__(64) void k_rank(const int32_t *__restrict__ ids, int32_t n, int64_t n_rows,
-                                             uint32_t *__restrict__ key_out, int32_t *__restrict__ pos_out)
+__global__ __launch_bounds__(256) void k_rank(const int32_t *__restrict__ ids, int32_t n, int64_t n_rows, uint2 *__restrict__ sorted)
 {
     __shared__ __attribute__((aligned(16))) uint32_t keys[RANK_MAX];
-    const int lane = threadIdx.x;
-    const int n4 = (n + 3) & ~3;
-    for (int i = lane; i < n4; i += 64) keys[i] = i < n ? sort_key(ids[i], n_rows) : 0xffffffffu;
+    const int n4 = (n + 3) & ~3, part = threadIdx.x & 15;
+    for (int i = threadIdx.x; i < n4; i += 256) keys[i] = i < n ? sort_key(ids[i], n_rows) : 0xffffffffu;
     __syncthreads();
-    const int t = blockIdx.x * 64 + lane;
+    const int t = blockIdx.x * 16 + (threadIdx.x >> 4);
     const uint32_t mine = keys[t < n ? t : 0];
     int32_t rank = 0;
-    for (int i = 0; i < n4; i += 4) {
+    for (int i = 4 * part; i < n4; i += 64) {
         const uint4 k = *(const uint4 *)(keys + i);
-        rank += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
-        rank += (k.x == mine && i < t) + (k.y == mine && i + 1 < t) + (k.z == mine && i + 2 < t) + (k.w == mine && i + 3 < t);
+        const uint32_t below = mine + (i + 3 < t);              // in front of t equal keys count as smaller
+        rank += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+        if (i <= t && t <= i + 3) rank += (k.x == mine && i < t) + (k.y == mine && i + 1 < t) + (k.z == mine && i + 2 < t);
     }
-    if (t < n) { key_out[rank] = mine; pos_out[rank] = t; }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) rank += __shfl_xor(rank, m, 16);
+    if (t < n && part == 0) sorted[rank] = make_uint2(mine, (uint32_t)t);
 }
 
 // Large batches: least significant digit first, DIGIT bits a pass, stable.  A tile is SORT_TILE consecutive entries of one
 // workgroup; a pass counts every tile's digits, turns the counts into first places and moves the entries.
-constexpr int SORT_TILE = 4096, SORT_BINS = 1024, SORT_PER = SORT_TILE / 256;
+// An entry is (key, position).
+constexpr int SORT_BINS = 1024;
 
-__global__ __launch_bounds__(256) void k_sort_count(const uint32_t *__restrict__ key, const int32_t *__restrict__ ids, int32_t n,
+template <int PER>
+__global__ __launch_bounds__(256) void k_sort_count(const uint2 *__restrict__ in, const int32_t *__restrict__ ids, int32_t n,
                                                     int64_t n_rows, int shift, int bins, int32_t *__restrict__ counts)
 {
     __shared__ int32_t cnt[SORT_BINS];
     for (int b = threadIdx.x; b < bins; b += 256) cnt[b] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
-    for (int i = 0; i < SORT_PER; ++i) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * PER);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         const int64_t t = base + i * 256 + threadIdx.x;
         if (t < n) {
-            const uint32_t k = ids ? sort_key(ids[t], n_rows) : key[t];
+            const uint32_t k = ids ? sort_key(ids[t], n_rows) : in[t].x;
             atomicAdd(&cnt[(k >> shift) & (bins - 1)], 1);          // whole numbers: any order gives the same count
         }
     }
@@ -126,10 +137,10 @@ __global__ __launch_bounds__(64) void k_sort_tiles(int32_t *__restrict__ counts,
     if (lane == 0) totals[blockIdx.x] = carry;
 }
 
-__global__ __launch_bounds__(256) void k_sort_move(const uint32_t *__restrict__ key, const int32_t *__restrict__ pos,
-                                                   const int32_t *__restrict__ ids, int32_t n, int64_t n_rows, int shift, int bits,
-                                                   const int32_t *__restrict__ counts, const int32_t *__restrict__ totals,
-                                                   uint32_t *__restrict__ key_out, int32_t *__restrict__ pos_out)
+template <int PER>
+__global__ __launch_bounds__(256) void k_sort_move(const uint2 *__restrict__ in, const int32_t *__restrict__ ids, int32_t n, int64_t n_rows,
+                                                   int shift, int bits, const int32_t *__restrict__ counts,
+                                                   const int32_t *__restrict__ totals, uint2 *__restrict__ out)
 {
     __shared__ int32_t cnt[4][SORT_BINS];
     __shared__ int32_t first[SORT_BINS];
@@ -155,19 +166,25 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint32_t *__restrict__ 
         for (int i = 0; i < 4; ++i) { if (4 * tid + i < bins) first[4 * tid + i] = at; at += c[i]; }
     }
     __syncthreads();
-    // a wave takes SORT_TILE / 4 consecutive entries, 64 at a time: a lane's place among the wave's entries of its bin
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE + wave * (SORT_TILE / 4);
-    uint32_t k[SORT_PER];
-    int32_t p[SORT_PER], r[SORT_PER];
+    // a wave takes 64 PER consecutive entries, 64 at a time: a lane's place among the wave's entries of its bin
+    const int64_t base = (int64_t)blockIdx.x * (256 * PER) + wave * (64 * PER);
+    uint32_t k[PER];
+    int32_t p[PER], r[PER];
 #pragma unroll
-    for (int i = 0; i < SORT_PER; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const int64_t t = base + i * 64 + lane;
         const bool live = t < n;
-        k[i] = live ? (ids ? sort_key(ids[t], n_rows) : key[t]) : 0;
-        p[i] = live ? (ids ? (int32_t)t : pos[t]) : -1;
+        if (ids) {
+            k[i] = live ? sort_key(ids[t], n_rows) : 0;
+            p[i] = live ? (int32_t)t : -1;
+        } else {
+            const uint2 e = live ? in[t] : make_uint2(0u, ~0u);
+            k[i] = e.x;
+            p[i] = (int32_t)e.y;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < SORT_PER; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const uint32_t bin = (k[i] >> shift) & (bins - 1);
         uint64_t same = __ballot(p[i] >= 0);
         for (int b = 0; b < bits; ++b) {
@@ -191,90 +208,107 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint32_t *__restrict__ 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < SORT_PER; ++i)
+    for (int i = 0; i < PER; ++i)
         if (p[i] >= 0) {
             const int32_t at = cnt[wave][(k[i] >> shift) & (bins - 1)] + r[i];
-            key_out[at] = k[i];
-            pos_out[at] = p[i];
+            out[at] = make_uint2(k[i], (uint32_t)p[i]);
         }
 }
 
-// first[v] = number of sorted keys below v, v = 0 .. n_rows
-__global__ __launch_bounds__(256) void k_row_first(const uint32_t *__restrict__ key, int32_t n, int64_t n_rows, int32_t *__restrict__ first)
+// number of sorted keys below v
+__device__ __forceinline__ int32_t first_of(const uint2 *__restrict__ sorted, int32_t n, uint32_t v)
+{
+    int32_t lo = 0, hi = n;
+    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (sorted[mid].x < v) lo = mid + 1; else hi = mid; }
+    return lo;
+}
+
+// first[v] for v = 0 .. n_rows
+__global__ __launch_bounds__(256) void k_row_first(const uint2 *__restrict__ sorted, int32_t n, int64_t n_rows, int32_t *__restrict__ first)
 {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v > n_rows) return;
-    int32_t lo = 0, hi = n;
-    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (key[mid] < (uint32_t)v) lo = mid + 1; else hi = mid; }
-    first[v] = lo;
+    if (v <= n_rows) first[v] = first_of(sorted, n, (uint32_t)v);
 }
 
 // ------------------------------------------------------------------ sums
-// A row with more than HEAVY tokens is summed in stretches that start at multiples of HEAVY of the sorted list, so that many
-// groups share a popular row.  Such a row crosses a multiple of HEAVY, so a stretch holds at most two of them: the one it
-// starts with (slot 0) and another it ends with (slot 1).
-constexpr int HEAVY = 256;
+// A row with more than 2^hs tokens is summed in stretches that start at multiples of 2^hs of the sorted list, so that many
+// groups of lanes share a popular row.  Such a row crosses a multiple of 2^hs, so a stretch holds at most two of them: the one
+// it starts with (slot 0) and another it ends with (slot 1).  The same again, SUPER stretches at a time, for rows of more than
+// 2 SUPER stretches.
+constexpr int SUPER = 64;
 
-// Sum of grad[pos[s .. e)], columns c .. c + V of this lane; the group's L lanes read L positions at once and hand them round
+// Sum of grad[positions s .. e), columns c .. c + V of this lane; the group's L lanes read L positions at once and hand them round
 template <typename T, int V, int L>
-__device__ __forceinline__ void sum_rows(const T *__restrict__ grad, int64_t stride, const int32_t *__restrict__ pos, int32_t s,
+__device__ __forceinline__ void sum_rows(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t s,
                                          int32_t e, int32_t c, int32_t d, int gl, float (&acc)[V])
 {
-    const bool in = c < d;
+    const T *base = grad + (c < d ? c : 0);
     for (int32_t a = s; a < e; a += L) {
         const int m = std::min<int32_t>(L, e - a);
-        const int32_t mine = pos[a + (gl < m ? gl : 0)];
+        const int32_t mine = (int32_t)sorted[a + (gl < m ? gl : 0)].y;
         int j = 0;
-        for (; j + 4 <= m; j += 4) {
-            float v[4][V];
+        for (; j + 8 <= m; j += 8) {
+            float v[8][V];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int32_t p = __shfl(mine, j + i, L);
-                load_vec<V>(grad + (int64_t)p * stride + (in ? c : 0), v[i]);
-            }
+            for (int i = 0; i < 8; ++i) load_vec<V>(base + (int64_t)__shfl(mine, j + i, L) * stride, v[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int q = 0; q < V; ++q) acc[q] += v[i][q];
         }
-        for (; j < m; ++j) {
-            float v[V];
-            const int32_t p = __shfl(mine, j, L);
-            load_vec<V>(grad + (int64_t)p * stride + (in ? c : 0), v);
+        if (j < m) {                    // up to seven more, asked for at once
+            float v[7][V];
 #pragma unroll
-            for (int q = 0; q < V; ++q) acc[q] += v[q];
+            for (int i = 0; i < 7; ++i) {
+                const int32_t p = __shfl(mine, j + i < m ? j + i : j, L);
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[i][q] = 0.f;
+                if (j + i < m) load_vec<V>(base + (int64_t)p * stride, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+#pragma unroll
+                for (int q = 0; q < V; ++q) acc[q] += v[i][q];
         }
     }
 }
 
-__device__ __forceinline__ int32_t first_of(const uint32_t *__restrict__ key, int32_t n, uint32_t v)
+// the row's parts k0 .. k1, of which the first is in slot 1 if the row starts inside it
+template <int V>
+__device__ __forceinline__ void sum_parts(const float *__restrict__ parts, int32_t k0, int32_t k1, int64_t start, int64_t width, int32_t c,
+                                          int32_t d, float (&acc)[V])
 {
-    int32_t lo = 0, hi = n;
-    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (key[mid] < v) lo = mid + 1; else hi = mid; }
-    return lo;
+    const float *src = parts + ((int64_t)k0 * 2 + ((int64_t)k0 * width < start)) * d + c;
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] += src[q];
+    src = parts + (int64_t)k0 * 2 * d + c;
+    const int32_t m = k1 - k0;
+#pragma unroll 8
+    for (int32_t k = 1; k <= m; ++k)
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] += src[(int64_t)k * 2 * d + q];
 }
 
 template <typename T, int V, int L>
-__global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad, int64_t stride, const uint32_t *__restrict__ key,
-                                                     const int32_t *__restrict__ pos, int32_t n, int64_t n_rows, int32_t d,
-                                                     const int32_t *__restrict__ first, float *__restrict__ parts)
+__global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t n,
+                                                     int64_t n_rows, int32_t d, const int32_t *__restrict__ first, int hs, float *__restrict__ parts)
 {
     const int gl = threadIdx.x % L;
     const int32_t chunk = (int32_t)((int64_t)blockIdx.x * (256 / L) + threadIdx.x / L);
-    const int64_t lo = (int64_t)chunk * HEAVY;
+    const int64_t lo = (int64_t)chunk << hs;
     if (lo >= n) return;
-    const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + HEAVY);
-    const uint32_t kf = key[a], kl = key[z - 1];
+    const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + (1 << hs));
+    const uint32_t kf = sorted[a].x, kl = sorted[z - 1].x;
 #pragma unroll 1
     for (int slot = 0; slot < 2; ++slot) {
         const uint32_t kk = slot ? kl : kf;
         if ((slot && kl == kf) || kk >= (uint64_t)n_rows) continue;
-        const int32_t s = first ? first[kk] : first_of(key, n, kk), e = first ? first[kk + 1] : first_of(key, n, kk + 1);
-        if (e - s <= HEAVY) continue;
+        const int32_t s = first ? first[kk] : first_of(sorted, n, kk), e = first ? first[kk + 1] : first_of(sorted, n, kk + 1);
+        if (e - s <= 1 << hs) continue;
         for (int32_t c0 = 0; c0 < d; c0 += V * L) {
             const int32_t c = c0 + gl * V;
             float acc[V] = {};
-            sum_rows<T, V, L>(grad, stride, pos, std::max(s, a), std::min(e, z), c, d, gl, acc);
+            sum_rows<T, V, L>(grad, stride, sorted, std::max(s, a), std::min(e, z), c, d, gl, acc);
             if (c < d) {
                 float *dst = parts + ((int64_t)chunk * 2 + slot) * d + c;
 #pragma unroll
@@ -284,42 +318,115 @@ __global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad,
     }
 }
 
-template <typename T, int V, int L>
-__global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, int64_t stride, const uint32_t *__restrict__ key,
-                                                  const int32_t *__restrict__ pos, int32_t n, int64_t n_rows, int32_t d, float scale,
-                                                  const int32_t *__restrict__ first, const float *__restrict__ parts, int accumulate,
+__device__ __forceinline__ int32_t stretches(int32_t s, int32_t e, int hs) { return ((e - 1) >> hs) - (s >> hs) + 1; }
+
+// one workgroup a super-stretch of SUPER parts; a thread a column
+__global__ __launch_bounds__(256) void k_super_parts(const uint2 *__restrict__ sorted, int32_t n, int64_t n_rows, int32_t d,
+                                                     const int32_t *__restrict__ first, int hs, const float *__restrict__ parts, float *__restrict__ supers)
+{
+    const int64_t lo = (int64_t)blockIdx.x * (SUPER << hs);
+    const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + (SUPER << hs));
+    const uint32_t kf = sorted[a].x, kl = sorted[z - 1].x;
+    for (int slot = 0; slot < 2; ++slot) {
+        const uint32_t kk = slot ? kl : kf;
+        if ((slot && kl == kf) || kk >= (uint64_t)n_rows) continue;
+        const int32_t s = first ? first[kk] : first_of(sorted, n, kk), e = first ? first[kk + 1] : first_of(sorted, n, kk + 1);
+        if (stretches(s, e, hs) <= 2 * SUPER) continue;
+        for (int32_t c = threadIdx.x; c < d; c += 256) {
+            float acc[1] = {};
+            sum_parts<1>(parts, std::max(s, a) >> hs, (std::min(e, z) - 1) >> hs, s, 1 << hs, c, d, acc);
+            supers[((int64_t)blockIdx.x * 2 + slot) * d + c] = acc[0];
+        }
+    }
+}
+
+// A group of L lanes sums R neighbouring rows, whose tokens are neighbours in the sorted list: one wait for the rows' first
+// places, one for the tokens' positions and one for every eight gradient rows, whichever row they belong to - a table row has
+// two or three tokens where the batch is as long as the table, and a wait a step and row would be most of the time.
+template <typename T, int V, int L, int R>
+__global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t n,
+                                                  int64_t n_rows, int32_t d, float scale, const int32_t *__restrict__ first, int hs,
+                                                  const float *__restrict__ parts, const float *__restrict__ supers, int accumulate,
                                                   T *__restrict__ out, int64_t out_stride)
 {
     const int gl = threadIdx.x % L;
-    const int64_t v = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (v >= n_rows) return;
-    const int32_t s = first ? first[v] : first_of(key, n, (uint32_t)v), e = first ? first[v + 1] : first_of(key, n, (uint32_t)v + 1);
-    if (s == e && accumulate) return;
+    const int64_t v0 = ((int64_t)blockIdx.x * (256 / L) + threadIdx.x / L) * R;
+    if (v0 >= n_rows) return;
+    const int rows = (int)std::min<int64_t>(R, n_rows - v0);
+    const int64_t vf = v0 + std::min(gl, rows);
+    const int32_t f = first ? first[vf] : first_of(sorted, n, (uint32_t)vf);
+    const int32_t f_next = __shfl(f, gl < R ? gl + 1 : R, L);
+    int heavy = gl < rows && f_next - f > 1 << hs;
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1) heavy |= __shfl_xor(heavy, m, L);
+    const int32_t s0 = __shfl(f, 0, L), e0 = __shfl(f, rows, L);
     for (int32_t c0 = 0; c0 < d; c0 += V * L) {
         const int32_t c = c0 + gl * V;
         float acc[V] = {};
-        if (e - s <= HEAVY) sum_rows<T, V, L>(grad, stride, pos, s, e, c, d, gl, acc);
-        else if (c < d)
-            for (int32_t k = s / HEAVY; k <= (e - 1) / HEAVY; ++k) {
-                const float *src = parts + ((int64_t)k * 2 + ((int64_t)k * HEAVY < s)) * d + c;
+        auto put = [&](int r, bool any) {
+            if (c < d && (any || !accumulate)) {
+                T *dst = out + (v0 + r) * out_stride + c;
+                float was[V] = {};
+                if (accumulate) load_vec<V>(dst, was);
 #pragma unroll
-                for (int q = 0; q < V; ++q) acc[q] += src[q];
+                for (int q = 0; q < V; ++q) was[q] = fmaf(acc[q], scale, was[q]);
+                store_vec<V>(dst, was);
             }
-        if (c < d) {
-            T *dst = out + v * out_stride + c;
-            float was[V] = {};
-            if (accumulate) load_vec<V>(dst, was);
 #pragma unroll
-            for (int q = 0; q < V; ++q) acc[q] = fmaf(acc[q], scale, was[q]);
-            store_vec<V>(dst, acc);
+            for (int q = 0; q < V; ++q) acc[q] = 0.f;
+        };
+        if (heavy) {
+            for (int r = 0; r < rows; ++r) {
+                const int32_t s = __shfl(f, r, L), e = __shfl(f, r + 1, L);
+                if (e - s <= 1 << hs) sum_rows<T, V, L>(grad, stride, sorted, s, e, c, d, gl, acc);
+                else if (c < d) {
+                    if (stretches(s, e, hs) <= 2 * SUPER) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc);
+                    else sum_parts<V>(supers, s / (SUPER << hs), (e - 1) / (SUPER << hs), s, SUPER << hs, c, d, acc);
+                }
+                put(r, e > s);
+            }
+            continue;
+        }
+        const T *base = grad + (c < d ? c : 0);
+        int r = 0;
+        int32_t s = s0, e = __shfl(f, 1, L);                 // of the row in work
+        for (int32_t a = s0; a < e0; a += L) {
+            const int m = std::min<int32_t>(L, e0 - a);
+            const int32_t mine = (int32_t)sorted[a + (gl < m ? gl : 0)].y;
+            for (int j = 0; j < m; j += 8) {
+                float v[8][V];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int32_t p = __shfl(mine, j + i < m ? j + i : j, L);
+                    if (j + i < m) load_vec<V>(base + (int64_t)p * stride, v[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (j + i < m) {
+                        while (a + j + i >= e) {             // behind the row: it is done, and so are empty ones after it
+                            put(r, e > s);
+                            ++r;
+                            s = e;
+                            e = __shfl(f, r + 1, L);
+                        }
+#pragma unroll
+                        for (int q = 0; q < V; ++q) acc[q] += v[i][q];
+                    }
+            }
+        }
+        for (; r < rows; ++r) {
+            put(r, e > s);
+            s = e;
+            e = __shfl(f, r + 2 <= rows ? r + 2 : rows, L);
         }
     }
 }
 
 // what a gradient call keeps in its workspace
 struct GradPlan {
-    int passes, bits, tiles;
-    int64_t key[2], pos[2], counts, totals, first, parts, bytes;
+    int passes, bits, per, tiles, hs;
+    bool first_table;
+    int64_t sorted[2], counts, totals, first, parts, supers, bytes;
 };
 
 GradPlan grad_plan(int64_t n, int64_t n_rows, int32_t d)
@@ -328,48 +435,74 @@ GradPlan grad_plan(int64_t n, int64_t n_rows, int32_t d)
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
     const bool small = n <= RANK_MAX;
-    for (int i = 0; i < (small ? 1 : 2); ++i) { p.key[i] = take(n * 4); p.pos[i] = take(n * 4); }
+    for (int i = 0; i < (small ? 1 : 2); ++i) p.sorted[i] = take(n * 8);
     if (!small) {
         int bits = 1;
         while (bits < 31 && (n_rows >> bits)) ++bits;       // keys are 0 .. n_rows
         p.passes = (bits + 9) / 10;
         p.bits = (bits + p.passes - 1) / p.passes;
-        p.tiles = (int)((n + SORT_TILE - 1) / SORT_TILE);
+        // small tiles fill the chip, large ones keep the table of counts short: the change is where either has a tile a CU
+        p.per = n <= 256 * 1024 ? 4 : 16;
+        p.tiles = (int)((n + 256 * p.per - 1) / (256 * p.per));
         p.counts = take((int64_t)(1 << p.bits) * p.tiles * 4);
         p.totals = take((int64_t)(1 << p.bits) * 4);
-        p.first = take((n_rows + 1) * 4);
     }
-    if (n > HEAVY) p.parts = take((n + HEAVY - 1) / HEAVY * 2 * (int64_t)d * 4);
+    // a table of the rows' first places, or (few rows) a search by every group that needs one
+    p.first_table = !small || n_rows > 65536;
+    if (p.first_table) p.first = take((n_rows + 1) * 4);
+    // Short stretches keep the wait for a popular row short (131072 tokens of bf16, d = 128: 74 us with 16, 85 with 32, 102
+    // with 64), long ones write and read fewer parts (2 M tokens of fp32: 432, 405 and 402 us)
+    p.hs = n <= 256 * 1024 ? 4 : 5;
+    if (n > 1 << p.hs) p.parts = take(((n + (1 << p.hs) - 1) >> p.hs) * 2 * (int64_t)d * 4);
+    if (n > 2 * SUPER << p.hs) p.supers = take((n + (SUPER << p.hs) - 1) / (SUPER << p.hs) * 2 * (int64_t)d * 4);
     p.bytes = std::max<int64_t>(at, 256);
     return p;
 }
 
+template <typename T> struct SumArgs {
+    const T *grad;
+    int64_t stride;
+    const uint2 *sorted;
+    int32_t n;
+    int64_t n_rows;
+    int32_t d;
+    float scale;
+    int accumulate;
+    const int32_t *first;
+    int hs;
+    float *parts, *supers;
+    T *out;
+    int64_t out_stride;
+};
+
 template <typename T, int V, int L>
-int launch_sums(const T *grad, int64_t stride, const uint32_t *key, const int32_t *pos, int32_t n, int64_t n_rows, int32_t d,
-                float scale, int accumulate, const int32_t *first, float *parts, T *out, int64_t out_stride, hipStream_t st)
+int launch_sums(const SumArgs<T> &a, hipStream_t st)
 {
     constexpr int G = 256 / L;
-    if (n > HEAVY) {
-        const int64_t chunks = ((int64_t)n + HEAVY - 1) / HEAVY;
-        hipLaunchKernelGGL((k_heavy_parts<T, V, L>), dim3((unsigned)((chunks + G - 1) / G)), dim3(256), 0, st, grad, stride, key, pos, n, n_rows, d,
-                           first, parts);
+    if (a.n > 1 << a.hs) {
+        const int64_t chunks = ((int64_t)a.n + (1 << a.hs) - 1) >> a.hs;
+        hipLaunchKernelGGL((k_heavy_parts<T, V, L>), dim3((unsigned)((chunks + G - 1) / G)), dim3(256), 0, st, a.grad, a.stride, a.sorted, a.n,
+                           a.n_rows, a.d, a.first, a.hs, a.parts);
+        if (a.n > 2 * SUPER << a.hs)
+            hipLaunchKernelGGL(k_super_parts, dim3((unsigned)((chunks + SUPER - 1) / SUPER)), dim3(256), 0, st, a.sorted, a.n, a.n_rows, a.d,
+                               a.first, a.hs, (const float *)a.parts, a.supers);
     }
-    hipLaunchKernelGGL((k_row_sums<T, V, L>), dim3((unsigned)((n_rows + G - 1) / G)), dim3(256), 0, st, grad, stride, key, pos, n, n_rows, d, scale,
-                       first, parts, accumulate, out, out_stride);
+    constexpr int R = L >= 16 ? 8 : 4, per_group = G * R;           // rows a group, rows a workgroup
+    hipLaunchKernelGGL((k_row_sums<T, V, L, R>), dim3((unsigned)((a.n_rows + per_group - 1) / per_group)), dim3(256), 0, st, a.grad, a.stride,
+                       a.sorted, a.n, a.n_rows, a.d, a.scale, a.first, a.hs, (const float *)a.parts, (const float *)a.supers, a.accumulate, a.out,
+                       a.out_stride);
     MF_LAUNCH_CHECK();
     return MFSGD_OK;
 }
 
 template <typename T, int V>
-int launch_sums_v(int lanes, const T *grad, int64_t stride, const uint32_t *key, const int32_t *pos, int32_t n, int64_t n_rows,
-                  int32_t d, float scale, int accumulate, const int32_t *first, float *parts, T *out, int64_t out_stride, hipStream_t st)
+int launch_sums_v(const SumArgs<T> &a, hipStream_t st)
 {
-#define MF_SUM(L_) return launch_sums<T, V, L_>(grad, stride, key, pos, n, n_rows, d, scale, accumulate, first, parts, out, out_stride, st)
-    if (lanes <= 8) MF_SUM(8);
-    if (lanes <= 16) MF_SUM(16);
-    if (lanes <= 32) MF_SUM(32);
-    MF_SUM(64);
-#undef MF_SUM
+    const int lanes = (a.d + V - 1) / V;
+    if (lanes <= 8) return launch_sums<T, V, 8>(a, st);
+    if (lanes <= 16) return launch_sums<T, V, 16>(a, st);
+    if (lanes <= 32) return launch_sums<T, V, 32>(a, st);
+    return launch_sums<T, V, 64>(a, st);
 }
 
 template <typename T>
@@ -377,38 +510,39 @@ int grad_impl(const T *grad, int64_t stride, const int32_t *ids, int64_t n, int6
               T *out, int64_t out_stride, char *ws, hipStream_t st)
 {
     const GradPlan p = grad_plan(n, n_rows, d);
-    uint32_t *key[2] = {(uint32_t *)(ws + p.key[0]), (uint32_t *)(ws + p.key[1])};
-    int32_t *pos[2] = {(int32_t *)(ws + p.pos[0]), (int32_t *)(ws + p.pos[1])};
-    int32_t *first = nullptr;
+    uint2 *sorted[2] = {(uint2 *)(ws + p.sorted[0]), (uint2 *)(ws + p.sorted[1])};
     const int32_t m = (int32_t)n;
     int at = 0;
     if (n <= RANK_MAX) {
-        if (n) hipLaunchKernelGGL(k_rank, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, ids, m, n_rows, key[0], pos[0]);
+        if (n) hipLaunchKernelGGL(k_rank, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, ids, m, n_rows, sorted[0]);
     } else {
         int32_t *counts = (int32_t *)(ws + p.counts), *totals = (int32_t *)(ws + p.totals);
         for (int pass = 0; pass < p.passes; ++pass) {
-            const int shift = pass * p.bits, from = (pass + 1) & 1;
+            const int shift = pass * p.bits;
+            const uint2 *in = sorted[(pass + 1) & 1];
             at = pass & 1;
             const int32_t *src = pass ? nullptr : ids;
-            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(256), 0, st, key[from], src, m, n_rows, shift, 1 << p.bits, counts);
+            if (p.per == 4) hipLaunchKernelGGL(k_sort_count<4>, dim3(p.tiles), dim3(256), 0, st, in, src, m, n_rows, shift, 1 << p.bits, counts);
+            else hipLaunchKernelGGL(k_sort_count<16>, dim3(p.tiles), dim3(256), 0, st, in, src, m, n_rows, shift, 1 << p.bits, counts);
             hipLaunchKernelGGL(k_sort_tiles, dim3(1 << p.bits), dim3(64), 0, st, counts, p.tiles, totals);
-            hipLaunchKernelGGL(k_sort_move, dim3(p.tiles), dim3(256), 0, st, key[from], pos[from], src, m, n_rows, shift, p.bits, counts,
-                               totals, key[at], pos[at]);
+            if (p.per == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3(p.tiles), dim3(256), 0, st, in, src, m, n_rows, shift, p.bits,
+                                               (const int32_t *)counts, (const int32_t *)totals, sorted[at]);
+            else hipLaunchKernelGGL(k_sort_move<16>, dim3(p.tiles), dim3(256), 0, st, in, src, m, n_rows, shift, p.bits,
+                                    (const int32_t *)counts, (const int32_t *)totals, sorted[at]);
         }
-        first = (int32_t *)(ws + p.first);
-        hipLaunchKernelGGL(k_row_first, dim3((unsigned)((n_rows + 256) / 256)), dim3(256), 0, st, key[at], m, n_rows, first);
     }
-    float *parts = (float *)(ws + p.parts);
+    int32_t *first = p.first_table ? (int32_t *)(ws + p.first) : nullptr;
+    if (first)
+        hipLaunchKernelGGL(k_row_first, dim3((unsigned)((n_rows + 256) / 256)), dim3(256), 0, st, (const uint2 *)sorted[at], m, n_rows, first);
+    const SumArgs<T> a = {grad, stride, sorted[at], m, n_rows, d, scale, accumulate, first, p.hs, (float *)(ws + p.parts), (float *)(ws + p.supers),
+                          out, out_stride};
     const int v = vec_elems(sizeof(T), d, stride, out_stride, grad, out);
-    const int lanes = (d + v - 1) / v;
-#define MF_GRAD(V_) return launch_sums_v<T, V_>(lanes, grad, stride, key[at], pos[at], m, n_rows, d, scale, accumulate, first, parts, out, out_stride, st)
     if constexpr (sizeof(T) == 2) {
-        if (v == 8) MF_GRAD(8);
+        if (v == 8) return launch_sums_v<T, 8>(a, st);
     }
-    if (v == 4) MF_GRAD(4);
-    if (v == 2) MF_GRAD(2);
-    MF_GRAD(1);
-#undef MF_GRAD
+    if (v == 4) return launch_sums_v<T, 4>(a, st);
+    if (v == 2) return launch_sums_v<T, 2>(a, st);
+    return launch_sums_v<T, 1>(a, st);
 }
 
 }  // namespace
@@ -421,6 +555,7 @@ int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows,
     MF_ARG(n >= 0 && n_rows >= 0 && n_rows <= INT32_MAX && d >= 1 && table_stride >= d, "embedding: bad shape");
     MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "embedding: unknown dtype %d", dtype);
     if (n == 0) return MFSGD_OK;
+    MF_ARG(n <= ((int64_t)1 << 40) / d, "embedding: more than 2^40 elements");
     MF_ARG(ids && out && (table || n_rows == 0), "embedding: null pointer");
     if (dtype == MFSGD_F32)
         return launch_embedding<float>((const float *)table, table_stride, n_rows, d, ids, n, scale, (float *)out, as_stream(stream));

@@ -576,16 +576,18 @@ struct JoinArgs {
     float *loss, *lse, *row_init, *row_q, *row_g;     // row_init NULL: no gradients
 };
 
-// One wave a row: joins the parts of the items' axis, adds the target's own term and writes loss, lse, the row's dX and what
+// W waves a row (one, or four where there are many parts): joins the parts of the items' axis, adds the target's own term and writes loss, lse, the row's dX and what
 // pass 2 needs of the row.
-template <typename T>
-__global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__restrict__ x, const T *__restrict__ w, T *__restrict__ dx)
+template <typename T, int W>
+__global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T *__restrict__ x, const T *__restrict__ w, T *__restrict__ dx)
 {
+    __shared__ float sums[W][256];
     const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int32_t t = a.targets[r];
     const bool in = (uint32_t)t < (uint64_t)a.n_items;
     if (!in) {
+        if (wave) return;
         if (lane == 0) {
             a.loss[r] = a.lse[r] = t < 0 ? 0.f : NAN;
             if (a.row_init) { a.row_init[r] = -INFINITY; a.row_q[r] = 0.f; if (a.row_g) a.row_g[r] = 0.f; }
@@ -616,13 +618,13 @@ __global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__r
     const float log_all = near ? log1pf(others) : logf(all);
     const float loss = none ? INFINITY : (near ? log_all : log_all + (ref - z) * LN2);
     const float q = none ? 0.f : others / all;                 // 1 - p_t
-    if (lane == 0) {
+    if (lane == 0 && wave == 0) {
         a.loss[r] = loss;
         a.lse[r] = none ? -INFINITY : log_all + ref * LN2;
     }
     if (!a.row_init) return;
     const float g = a.weights ? a.weights[r] : 1.f;
-    if (lane == 0) {
+    if (lane == 0 && wave == 0) {
         a.row_init[r] = none ? -INFINITY : -((log_all + ref * LN2) / a.scale);
         a.row_q[r] = q * g;
         if (a.row_g) a.row_g[r] = none ? 0.f : g;
@@ -633,8 +635,8 @@ __global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__r
     const int c = lane % lanes * 4, step = 64 / lanes;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (c < a.dp) {
-#pragma unroll 4
-        for (int s = lane / lanes; s < a.splits; s += step) {
+#pragma unroll 8
+        for (int s = wave * step + lane / lanes; s < a.splits; s += W * step) {
             const float w2 = __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);
             const f32x4 p = *(const f32x4 *)(a.part_o + ((int64_t)s * a.n + r) * a.dp + c);
             v += p * w2;
@@ -643,6 +645,14 @@ __global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__r
     for (int k = lanes; k < 64; k <<= 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], k, 64);
+    if constexpr (W > 1) {
+        if (lane < lanes && c < a.dp) *(f32x4 *)(sums[wave] + c) = v;
+        __syncthreads();
+        if (wave) return;
+        if (lane < lanes && c < a.dp)
+#pragma unroll
+            for (int k = 1; k < W; ++k) v += *(const f32x4 *)(sums[k] + c);
+    }
     if (lane < lanes)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -652,19 +662,23 @@ __global__ __launch_bounds__(64) void k_join_rows(const JoinArgs a, const T *__r
             }
 }
 
-// the parts of the rows' axis of pass 2, summed in order: dW and db
+// the parts of the rows' axis of pass 2, summed in order: dW and db.  Four columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ part_o, const float *__restrict__ part_s, int32_t splits,
                                                     int64_t n_items, int32_t d, int32_t dp, float f, float weight, T *__restrict__ dw,
                                                     float *__restrict__ db)
 {
+    const int32_t per = (d + 3) / 4;
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p >= n_items * d) return;
-    const int64_t v = p / d;
-    const int32_t c = (int32_t)(p - v * d);
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part_o[((int64_t)k * n_items + v) * dp + c];
-    store_f32(dw + p, s * f);
+    if (p >= n_items * per) return;
+    const int64_t v = p / per;
+    const int32_t c = (int32_t)(p - v * per) * 4;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += *(const f32x4 *)(part_o + ((int64_t)k * n_items + v) * dp + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (c + i < d) store_f32(dw + v * d + c + i, s[i] * f);
     if (db && c == 0) {
         float t = 0.f;
         for (int k = 0; k < splits; ++k) t += part_s[(int64_t)k * n_items + v];
@@ -689,18 +703,22 @@ PassShape pass_shape(int dp, int mode, bool conv)
     return conv ? pass_shape_d<PL, TABLE, true>(dp) : pass_shape_d<PL, TABLE, false>(dp);
 }
 
-// Parts the streamed axis is cut into.  A workgroup's time counts in tiles (HEAD more for its start and end), the parts' sums
-// are written and read again (PART tiles a part, if a workgroup's share of memory were all it waited for): the number of
-// parts with the least rounds x (tiles + HEAD) + parts x PART.
-int parts_of(int64_t n_sm, int64_t row_tiles, const PassShape &s, double head, double part)
+// Parts the streamed axis is cut into: the number with the least time by this reckoning.  A workgroup takes 4 us to start and
+// end; a tile takes what its products take at the chip's measured rate (1000 TFLOP/s), shared by all workgroups at once; a
+// part's sums are written and read again at 4 TB/s; joining a part takes a row's wave a fraction of a wait for memory.
+int parts_of(int64_t n_sm, int64_t n_st, int64_t row_tiles, const PassShape &s, int dp, int products, bool sums)
 {
+    static const int counts[] = {1, 2, 3, 4, 5, 6, 7, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024};
+    const double tile_us = 2.0 * s.rows * s.tile * dp * products * s.groups * 1e-9;
+    const double part_us = (sums ? n_st * (double)dp * 8 / 4e6 : 0.0) + 0.015;
     const int64_t tiles = (n_sm + s.tile - 1) / s.tile;
     int best = 1;
     double least = 1e300;
-    for (int k = 1; k <= 1024 && k <= tiles; k += k < 8 ? 1 : 8 - k % 8) {
-        const int64_t rounds = (row_tiles * k + s.groups - 1) / s.groups;
-        const double cost = rounds * ((tiles + k - 1) / k + head) + (k > 1 ? k * part * rounds * s.groups / (row_tiles * k) : 0.0);
-        if (cost < least * 0.999) { least = cost; best = k; }
+    for (int k : counts) {
+        if (k > tiles) break;
+        const double rounds = (double)((row_tiles * k + s.groups - 1) / s.groups);
+        const double us = rounds * ((double)((tiles + k - 1) / k) * tile_us + 4.0) + (k > 1 ? k * part_us : 0.0);
+        if (us < least) { least = us; best = k; }
     }
     return best;
 }
@@ -724,9 +742,10 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     p.conv = n <= shape(mode1, true).rows && !(p.planes == 3 && p.dp == 256 && grads);
     const PassShape s1 = shape(mode1, p.conv), s2 = shape(TABLE, p.conv);
     p.rt1 = (int)((n + s1.rows - 1) / s1.rows);
-    p.splits1 = parts_of(n_items, p.rt1, s1, 2.0, 0.5);
+    const int six = p.planes == 3 ? 6 : 1;
+    p.splits1 = parts_of(n_items, n, p.rt1, s1, p.dp, six * (grads ? 2 : 1), grads);
     p.rt2 = (int)((n_items + s2.rows - 1) / s2.rows);
-    p.splits2 = parts_of(n, p.rt2, s2, 2.0, 1.0);
+    p.splits2 = parts_of(n, n_items, p.rt2, s2, p.dp, six * 2, true);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
     if (!p.conv) {
@@ -812,7 +831,9 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
         j.row_init = (float *)(ws + p.init); j.row_q = (float *)(ws + p.q);
         j.row_g = weights ? (float *)(ws + p.g) : nullptr;
     }
-    hipLaunchKernelGGL((k_join_rows<T>), dim3((unsigned)n), dim3(64), 0, st, j, x, w, dx);
+    // four waves a row: 192 parts of one row 12 -> 5 us; one wave where the rows fill the chip
+    if (grads && p.splits1 >= 32) hipLaunchKernelGGL((k_join_rows<T, 4>), dim3((unsigned)n), dim3(256), 0, st, j, x, w, dx);
+    else hipLaunchKernelGGL((k_join_rows<T, 1>), dim3((unsigned)n), dim3(64), 0, st, j, x, w, dx);
     MF_LAUNCH_CHECK();
     if (!grads) return MFSGD_OK;
 
@@ -830,7 +851,7 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     a.out_vec = vec_elems(sizeof(T), d, d, d, dw, dw);
     if (const int rc = launch_stream_d<T, TABLE>(p.dp, p.conv, a, st)) return rc;
     if (p.splits2 > 1) {
-        hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * d + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,
+        hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * ((d + 3) / 4) + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,
                            d, p.dp, scale * weight, weight, dw, db);
         MF_LAUNCH_CHECK();
     }

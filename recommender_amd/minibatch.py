@@ -58,10 +58,11 @@ class _On:
         self.guard = None
 
     def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
+        index = self.device.index
+        if index != torch.cuda.current_device():
             self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        self.stream = torch.cuda.current_stream().cuda_stream
+        self.stream = torch.cuda.current_stream(index).cuda_stream
         return self
 
     def __exit__(self, *exc):

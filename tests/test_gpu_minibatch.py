@@ -69,6 +69,8 @@ def test_embedding_shapes_and_alignment():
     assert torch.equal(ra.embedding(table.t().contiguous().t(), ids), table[ids.long()])       # columns contiguous
     assert torch.equal(ra.embedding(table[:1].expand(9, 16), ids % 9), table[:1].expand(2, 3, 4, 16))
     assert ra.embedding(table, ids[:0]).shape == (0, 3, 4, 16)
+    none = ra.embedding(table[:0], torch.tensor([-1, 0], dtype=torch.int32, device="cuda")).float()
+    assert float(none[0].abs().sum()) == 0 and bool(torch.isnan(none[1]).all())
     assert torch.equal(ra.embedding(table, ids.transpose(0, 2)), table[ids.transpose(0, 2).long()])
 
 
