@@ -35,9 +35,9 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-// The running maximum follows a tile's only when it rose by more than this (log2): any reference will do as long as
-// nothing overflows, and a new one costs a multiplication of all sums.
-constexpr float SLACK = 8.f;
+// The reference of a row's exponentials is the largest logit of the first 32 items that are in the catalogue, and stays it
+// while the row's sum is below this (log2 60): what counts is that nothing overflows, so no maximum is taken on the way.
+constexpr float TOO_MUCH = 1.152921504606846976e18f;
 
 enum { LOSS = 0, LOSS_SUMS = 1, TABLE = 2 };   // pass 1 without / with the weighted sums, pass 2
 
@@ -333,6 +333,12 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     for (int32_t t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1;
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
+        bool hit_tile = false;                          // does any row's target lie in this tile?
+        if constexpr (MODE != TABLE) {
+#pragma unroll
+            for (int u = 0; u < UT; ++u) hit_tile |= (uint32_t)(target[u] - t * TB) < (uint32_t)TB;
+            hit_tile = __ballot(hit_tile) != 0;
+        }
 #pragma unroll
         for (int sub = 0; sub < TB / 32; ++sub) {
             // logits (in units of scale) of 32 streamed rows: acc[u][j] is row 8 (j / 4) + 4 kh + j % 4 for stationary row `col`
@@ -381,32 +387,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             }
             bf16x8 w[UT][2][PL];       // the exponentials as operands: j 0..7 and 8..15
             uint32_t hits = 0, at = 0;
-            if constexpr (MODE != TABLE) {
-                float top[UT];
-                bool rise = false;
-#pragma unroll
-                for (int u = 0; u < UT; ++u) {
-                    float v = acc[u][0];
-#pragma unroll
-                    for (int j = 1; j < 16; ++j) v = fmaxf(v, acc[u][j]);
-                    const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-                    top[u] = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.c;
-                    rise |= top[u] > m[u] + SLACK;
-                }
-                if (__ballot(rise)) {
-#pragma unroll
-                    for (int u = 0; u < UT; ++u) {
-                        const bool mine = top[u] > m[u] + SLACK;
-                        const float f = mine ? __builtin_amdgcn_exp2f(m[u] - top[u]) : 1.f;    // the first tile: exp2(-inf) = 0
-                        if (mine) m[u] = top[u];
-                        sum[u] *= f;
-                        if constexpr (MODE == LOSS_SUMS) {
-#pragma unroll
-                            for (auto &v : o[u]) { v *= f; __builtin_amdgcn_sched_barrier(0); }
-                        }
-                    }
-                }
-            } else {
+            if constexpr (MODE == TABLE) {
                 // rows of the tile whose target is one of this wave's items
                 at = (uint32_t)(l_t[buf * TB + sub * 32 + col] - st0);
                 hits = (uint32_t)__ballot(at < 32u * UT);
@@ -415,14 +396,41 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             for (int u = 0; u < UT; ++u) {
                 float e[16];
                 if constexpr (MODE != TABLE) {
-                    const float ref = m[u] == -INFINITY ? 0.f : m[u];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, -ref));
                     const uint32_t own = (uint32_t)(target[u] - (t * TB + sub * 32));
-                    if (__ballot(own < 32u)) {
+                    float add;
+                    auto weigh = [&] {
+                        const float ref = m[u] == -INFINITY ? 0.f : m[u];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) e[j] = own == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
+                        for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, -ref));
+                        if (hit_tile) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) e[j] = own == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
+                        }
+                        float s4[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);
+                        add = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    };
+                    weigh();
+                    bool rise = m[u] == -INFINITY || sum[u] + add > TOO_MUCH;
+                    if (__ballot(rise)) {               // rare: a new reference, the same for both lanes of a row
+                        rise |= (bool)__shfl_xor((int)rise, 32, 64);
+                        float top = acc[u][0];
+#pragma unroll
+                        for (int j = 1; j < 16; ++j) top = fmaxf(top, acc[u][j]);
+                        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
+                        const float both = sum[u] + __shfl_xor(sum[u], 32, 64);
+                        const float up = both > 1.f ? fmaxf(top, m[u] + __builtin_amdgcn_logf(both)) : fmaxf(top, m[u]);
+                        const float f = rise && up > m[u] ? __builtin_amdgcn_exp2f(m[u] - up) : 1.f;     // the first time: exp2(-inf) = 0
+                        if (rise) m[u] = up;
+                        sum[u] *= f;
+                        if constexpr (MODE == LOSS_SUMS) {
+#pragma unroll
+                            for (auto &v : o[u]) { v *= f; __builtin_amdgcn_sched_barrier(0); }
+                        }
+                        weigh();
                     }
+                    sum[u] += add;
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, b2[u]));
@@ -449,7 +457,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                         }
                     }
                 }
-                if (MODE != TABLE || a.part_s) {
+                if (MODE == TABLE && a.part_s) {
                     float s4[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s4[j] = (e[j] + e[j + 4]) + (e[j + 8] + e[j + 12]);

@@ -11,6 +11,8 @@ The reference has no counterpart: it updates rating by rating.  All arguments ar
 bfloat16; ids and targets are int32, and a negative one is padding.  Every call runs on the current stream of that device
 without waiting for it, allocates through torch only, and can be captured into a graph.  Results are the same bits on every
 call.  There is no autograd: a gradient is its own call."""
+from array import array
+
 import torch
 
 from . import _abi
@@ -216,10 +218,17 @@ def _grad_set(tensors, name):
     return tensors
 
 
+def _addresses(tensors):
+    return array("Q", [t.data_ptr() for t in tensors])
+
+
 def _set_args(tensors):
-    n = len(tensors)
-    return ((_abi.c_vp * n)(*[t.data_ptr() for t in tensors]), (_abi.c_i64 * n)(*[t.numel() for t in tensors]),
-            (_abi.c_i32 * n)(*[_DTYPES[t.dtype] for t in tensors]))
+    """Host arrays of a set's addresses, sizes and types (to be kept alive until the call returns)."""
+    return _addresses(tensors), array("q", [t.numel() for t in tensors]), array("i", [_DTYPES[t.dtype] for t in tensors])
+
+
+def _at(a):
+    return a.buffer_info()[0]
 
 
 def grad_norm(tensors):
@@ -228,9 +237,9 @@ def grad_norm(tensors):
     with _On(*tensors) as on:
         norm = torch.empty((), dtype=torch.float32, device=on.device)
         ptrs, sizes, dtypes = _set_args(tensors)
-        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, len(tensors)))
-        _abi.check(_abi.lib().mfsgd_hip_grad_norm(ptrs, sizes, dtypes, len(tensors), norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                  on.stream))
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(_at(sizes), len(tensors)))
+        _abi.check(_abi.lib().mfsgd_hip_grad_norm(_at(ptrs), _at(sizes), _at(dtypes), len(tensors), norm.data_ptr(), ws.data_ptr(),
+                                                  ws.numel(), on.stream))
     return norm
 
 
@@ -248,8 +257,8 @@ def clip_grads(tensors, max_norm, out=None):
     with _On(*tensors, *(out or ())) as on:
         norm = torch.empty((), dtype=torch.float32, device=on.device)
         ptrs, sizes, dtypes = _set_args(tensors)
-        outs = None if out is None else _set_args(out)[0]
-        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, len(tensors)))
-        _abi.check(_abi.lib().mfsgd_hip_clip_grads(ptrs, outs, sizes, dtypes, len(tensors), max_norm, norm.data_ptr(),
-                                                   ws.data_ptr(), ws.numel(), on.stream))
+        outs = None if out is None else _addresses(out)
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(_at(sizes), len(tensors)))
+        _abi.check(_abi.lib().mfsgd_hip_clip_grads(_at(ptrs), None if outs is None else _at(outs), _at(sizes), _at(dtypes),
+                                                   len(tensors), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
     return norm
