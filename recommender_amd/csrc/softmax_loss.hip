@@ -38,6 +38,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // The reference of a row's exponentials is the largest logit of the first 32 items that are in the catalogue, and stays it
 // while the row's sum is below this (log2 60): what counts is that nothing overflows, so no maximum is taken on the way.
 constexpr float TOO_MUCH = 1.152921504606846976e18f;
+constexpr float UNSET = 1e30f;          // the sum of a row that has no reference yet: too much, so that the next items set one
 
 enum { LOSS = 0, LOSS_SUMS = 1, TABLE = 2 };   // pass 1 without / with the weighted sums, pass 2
 
@@ -131,14 +132,10 @@ __device__ __forceinline__ void split_piece(const Piece<float> &in, bool live, b
     }
 }
 
-#ifndef UTX
-#define UTX (PL == 3 || CONV || (MODE != LOSS && DP > 64) ? 1 : 2)
-#endif
-#ifndef RX
-#define RX 48
-#endif
 template <int DP, int PL, int MODE, bool CONV> struct Shape {
-    static constexpr int UT = UTX;                                   // 32-row tiles of stationary rows a wave keeps
+    // 32-row tiles of stationary rows a wave keeps.  Two halve the reads of LDS, which bound nothing but the loss of wide bf16
+    // rows (4096 x 59047, d = 256: 122 us with two, 130 with one); elsewhere one leaves more waves a SIMD
+    static constexpr int UT = PL == 1 && !CONV && MODE == LOSS && DP > 128 ? 2 : 1;
     static constexpr int ROWS = 128 * UT;                            // stationary rows a workgroup
     static constexpr int NB = DP == 256 && MODE != LOSS ? (PL == 1 ? 8 : 4) : 0;     // sixteenths of a stationary row that wait in LDS
     static constexpr int TB = ((PL == 3 || CONV) && DP > 32) || NB ? 32 : 64;      // streamed rows a tile
@@ -147,7 +144,7 @@ template <int DP, int PL, int MODE, bool CONV> struct Shape {
     static constexpr int LDS = 2 * BUF + 2 * TB * 16 + NB * PL * 4096;
     static constexpr int HOLD = CONV ? TB * CH / 256 : 0;            // pieces a thread holds on their way to LDS
     // registers: the stationary rows, the sums, the logits and what is in flight
-    static constexpr int REGS = UT * PL * (DP - 16 * NB) / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + HOLD * (PL == 3 ? 8 : 4) + (CONV ? 20 : 0) + RX;
+    static constexpr int REGS = UT * PL * (DP - 16 * NB) / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + HOLD * (PL == 3 ? 8 : 4) + (CONV ? 20 : 0) + 48;
     static constexpr int WAVES = REGS <= 120 ? 4 : REGS <= 156 ? 3 : REGS <= 256 ? 2 : 1;        // a SIMD
     static constexpr int GROUPS = WAVES < 160 * 1024 / LDS ? WAVES : 160 * 1024 / LDS;           // workgroups a CU
 };
@@ -168,10 +165,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     using S = Shape<DP, PL, MODE, CONV>;
     constexpr int UT = S::UT, TB = S::TB, CH = S::CH, BUF = S::BUF, KS = DP / 16, DT = DP / 32, PLANE = TB * DP * 2;
     constexpr int Q = BUF / 4096, HOLD = S::HOLD;
-#ifndef GAX
-#define GAX (PL == 3 ? 1 : 2)
-#endif
-    constexpr int GA = GAX;
+    constexpr int GA = PL == 3 ? 1 : 2;                 // operands of a group
     static_assert(BUF % 4096 == 0, "a tile is a whole number of 1 KB pieces per wave");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *l_init = (float *)(lds + 2 * BUF);           // [2][TB]
@@ -289,11 +283,12 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     };
 
     f32x16 o[UT][MODE == LOSS ? 1 : DT];
-    float m[UT], sum[UT];
+    float m[UT], neg_ref[UT], sum[UT];              // log2 reference, -reference as the exponent takes it, sum
 #pragma unroll
     for (int u = 0; u < UT; ++u) {
         m[u] = -INFINITY;
-        sum[u] = 0.f;
+        neg_ref[u] = 0.f;
+        sum[u] = MODE == TABLE ? 0.f : UNSET;
 #pragma unroll
         for (auto &v : o[u]) v = (f32x16)(0.f);
     }
@@ -351,6 +346,8 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             }
 #pragma unroll
             for (int u = 1; u < UT; ++u) acc[u] = acc[0];
+            // the wave that multiplies goes first: the others' exponentials fill its gaps (8192 x 17770 x 128 fp32: 786 -> 764 us)
+            __builtin_amdgcn_s_setprio(1);
             // operands are read one group ahead of the products that take them
             bf16x8 x[2][GA][PL];
 #pragma unroll
@@ -385,6 +382,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 #pragma unroll
                 for (int q = 0; q < GA; ++q) load_t(sub, q, x[0][q]);
             }
+            __builtin_amdgcn_s_setprio(0);
             bf16x8 w[UT][2][PL];       // the exponentials as operands: j 0..7 and 8..15
             uint32_t hits = 0, at = 0;
             if constexpr (MODE == TABLE) {
@@ -396,15 +394,15 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             for (int u = 0; u < UT; ++u) {
                 float e[16];
                 if constexpr (MODE != TABLE) {
-                    const uint32_t own = (uint32_t)(target[u] - (t * TB + sub * 32));
                     float add;
                     auto weigh = [&] {
-                        const float ref = m[u] == -INFINITY ? 0.f : m[u];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, -ref));
+                        for (int j = 0; j < 16; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(acc[u][j], a.c, neg_ref[u]));
                         if (hit_tile) {
+                            int32_t own = target[u] - (t * TB + sub * 32) - 4 * kh;
+                            asm volatile("" : "+v"(own));           // keeps the 16 comparisons inside the branch
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) e[j] = own == (uint32_t)(8 * (j / 4) + 4 * kh + j % 4) ? 0.f : e[j];
+                            for (int j = 0; j < 16; ++j) e[j] = own == 8 * (j / 4) + j % 4 ? 0.f : e[j];
                         }
                         float s4[4];
 #pragma unroll
@@ -412,9 +410,10 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                         add = (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     };
                     weigh();
-                    bool rise = m[u] == -INFINITY || sum[u] + add > TOO_MUCH;
+                    bool rise = sum[u] + add > TOO_MUCH;
                     if (__ballot(rise)) {               // rare: a new reference, the same for both lanes of a row
                         rise |= (bool)__shfl_xor((int)rise, 32, 64);
+                        if (m[u] == -INFINITY && sum[u] == UNSET) sum[u] = 0.f;
                         float top = acc[u][0];
 #pragma unroll
                         for (int j = 1; j < 16; ++j) top = fmaxf(top, acc[u][j]);
@@ -428,7 +427,9 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 #pragma unroll
                             for (auto &v : o[u]) { v *= f; __builtin_amdgcn_sched_barrier(0); }
                         }
+                        neg_ref[u] = m[u] == -INFINITY ? 0.f : -m[u];
                         weigh();
+                        if (m[u] == -INFINITY && sum[u] == 0.f && add == 0.f) sum[u] = UNSET;     // still no item in the catalogue
                     }
                     sum[u] += add;
                 } else {
@@ -517,6 +518,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 #pragma unroll
     for (int u = 0; u < UT; ++u) {
         const int32_t row = st0 + 32 * u + col;
+        if (MODE != TABLE && sum[u] == UNSET) sum[u] = 0.f;
         const float both = sum[u] + __shfl_xor(sum[u], 32, 64);
         if (row >= n_st) continue;
         const int64_t out = (int64_t)split * n_st + row;
@@ -745,9 +747,10 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     p.planes = dtype == MFSGD_F32 ? 3 : 1;
     const int mode1 = grads ? LOSS_SUMS : LOSS;
     auto shape = [&](int mode, bool conv) { return p.planes == 3 ? pass_shape<3>(p.dp, mode, conv) : pass_shape<1>(p.dp, mode, conv); };
-    // with one row tile the items are read once either way: converting them on the way saves a launch and a round trip
-    // (fp32 rows of 256 with gradients leave no registers for it)
-    p.conv = n <= shape(mode1, true).rows && !(p.planes == 3 && p.dp == 256 && grads);
+    // Few row tiles convert the rows they stream on the way: a launch and a round trip to memory less (200 x 162541 x 64 fp32
+    // step: 150 -> 143 us; with 8 row tiles nothing is gained, with more it costs).  fp32 rows of 256 with gradients leave no
+    // registers for it.
+    p.conv = n <= 4 * shape(mode1, true).rows && !(p.planes == 3 && p.dp == 256 && grads);
     const PassShape s1 = shape(mode1, p.conv), s2 = shape(TABLE, p.conv);
     p.rt1 = (int)((n + s1.rows - 1) / s1.rows);
     const int six = p.planes == 3 ? 6 : 1;

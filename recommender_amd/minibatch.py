@@ -54,8 +54,9 @@ class _On:
     def __init__(self, *tensors):
         _abi.require_gpu()
         self.device = tensors[0].device
+        index = tensors[0].get_device()
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.device != self.device):
+            if t is not None and (t.get_device() != index or index < 0):
                 raise ValueError("all tensors must be on one ROCm device")
         self.guard = None
 
@@ -206,39 +207,36 @@ def _dense(t):
     return True
 
 
-def _grad_set(tensors, name):
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not tensors:
-        raise ValueError(f"{name} is empty")
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
-            raise TypeError(f"{name} must be float32 or bfloat16 tensors")
-        if t.numel() and not _dense(t):
-            raise ValueError(f"{name} must be dense tensors (no gaps, no element twice)")
-    return tensors
+class _Set:
+    """A set of tensors and the host arrays of their addresses, sizes and types (which live as long as it does)."""
 
+    def __init__(self, tensors, name):
+        self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        if not self.tensors:
+            raise ValueError(f"{name} is empty")
+        try:
+            self.dtypes = array("i", [_DTYPES[t.dtype] for t in self.tensors])
+        except (KeyError, AttributeError):
+            raise TypeError(f"{name} must be float32 or bfloat16 tensors") from None
+        self.sizes = array("q", [t.numel() for t in self.tensors])
+        for t in self.tensors:
+            if not t.is_contiguous() and t.numel() and not _dense(t):
+                raise ValueError(f"{name} must be dense tensors (no gaps, no element twice)")
+        self.addresses = array("Q", [t.data_ptr() for t in self.tensors])
+        self.n = len(self.tensors)
 
-def _addresses(tensors):
-    return array("Q", [t.data_ptr() for t in tensors])
-
-
-def _set_args(tensors):
-    """Host arrays of a set's addresses, sizes and types (to be kept alive until the call returns)."""
-    return _addresses(tensors), array("q", [t.numel() for t in tensors]), array("i", [_DTYPES[t.dtype] for t in tensors])
-
-
-def _at(a):
-    return a.buffer_info()[0]
+    def args(self):
+        return self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], self.n
 
 
 def grad_norm(tensors):
     """sqrt of the sum of all squares of all tensors (float32 and bfloat16 in any mix), as a float32 tensor of no dimensions."""
-    tensors = _grad_set(tensors, "tensors")
-    with _On(*tensors) as on:
+    grads = _Set(tensors, "tensors")
+    with _On(*grads.tensors) as on:
         norm = torch.empty((), dtype=torch.float32, device=on.device)
-        ptrs, sizes, dtypes = _set_args(tensors)
-        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(_at(sizes), len(tensors)))
-        _abi.check(_abi.lib().mfsgd_hip_grad_norm(_at(ptrs), _at(sizes), _at(dtypes), len(tensors), norm.data_ptr(), ws.data_ptr(),
+        sizes, dtypes, n = grads.args()
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, n))
+        _abi.check(_abi.lib().mfsgd_hip_grad_norm(grads.addresses.buffer_info()[0], sizes, dtypes, n, norm.data_ptr(), ws.data_ptr(),
                                                   ws.numel(), on.stream))
     return norm
 
@@ -246,19 +244,19 @@ def grad_norm(tensors):
 def clip_grads(tensors, max_norm, out=None):
     """Scales all tensors by min(1, max_norm / norm), norm being their global norm, in place or into `out` (tensors of the same
     shapes, types and strides).  Returns the norm before clipping, without waiting for it."""
-    tensors = _grad_set(tensors, "tensors")
+    grads = _Set(tensors, "tensors")
     if not max_norm > 0:
         raise ValueError("max_norm must be positive")
+    to = grads
     if out is not None:
-        out = _grad_set(out, "out")
-        if len(out) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.stride() != t.stride()
-                                           for o, t in zip(out, tensors)):
+        to = _Set(out, "out")
+        if to.n != grads.n or to.dtypes != grads.dtypes or any(
+                o.shape != t.shape or o.stride() != t.stride() for o, t in zip(to.tensors, grads.tensors)):
             raise ValueError("out must have a tensor like each of tensors")
-    with _On(*tensors, *(out or ())) as on:
+    with _On(*grads.tensors, *(to.tensors if to is not grads else ())) as on:
         norm = torch.empty((), dtype=torch.float32, device=on.device)
-        ptrs, sizes, dtypes = _set_args(tensors)
-        outs = None if out is None else _addresses(out)
-        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(_at(sizes), len(tensors)))
-        _abi.check(_abi.lib().mfsgd_hip_clip_grads(_at(ptrs), None if outs is None else _at(outs), _at(sizes), _at(dtypes),
-                                                   len(tensors), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
+        sizes, dtypes, n = grads.args()
+        ws = on.workspace(_abi.lib().mfsgd_grad_norm_workspace(sizes, n))
+        _abi.check(_abi.lib().mfsgd_hip_clip_grads(grads.addresses.buffer_info()[0], to.addresses.buffer_info()[0], sizes, dtypes, n,
+                                                   max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
     return norm
