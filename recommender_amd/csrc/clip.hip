@@ -112,17 +112,13 @@ template <typename T>
 __device__ __forceinline__ void piece_scale(const T *p, T *o, int64_t n, float factor)
 {
     constexpr int V = 16 / sizeof(T), U = 4;
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const bool wide = (uintptr_t)p % 16 == 0 && (uintptr_t)o % 16 == 0;
     const int64_t nv = wide ? n / V : 0, blocks = nv / (256 * U);
     for (int64_t i = nv * V + threadIdx.x; i < n; i += 256) store_f32(o + i, load_f32(p + i) * factor);
     auto scaled = [&](float (&v)[V], int64_t i) {
 #pragma unroll
         for (int q = 0; q < V; ++q) v[q] *= factor;
-        u32x4 w;
-        if constexpr (sizeof(T) == 4) w = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-        else w = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
-        __builtin_nontemporal_store(w, (u32x4 *)(o + i * V));
+        store_past<V>(o + i * V, v);
     };
     for (int64_t i = blocks * 256 * U + threadIdx.x; i < nv; i += 256) {
         float v[V];

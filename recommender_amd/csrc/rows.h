@@ -61,6 +61,29 @@ template <int N> __device__ __forceinline__ void store_vec(__bf16 *p, const floa
     }
 }
 
+// ... past the caches (V elements are 4, 8 or 16 bytes; one bf16 element goes through them)
+template <int N, typename T> __device__ __forceinline__ void store_past(T *p, const float (&v)[N])
+{
+    constexpr int W = N * sizeof(T) / 4;
+    if constexpr (W == 0) store_vec<N>(p, v);
+    else {
+        uint32_t w[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+            else w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        }
+        typedef uint32_t words __attribute__((ext_vector_type(W)));
+        words x;
+        if constexpr (W == 1) x = (words)w[0];
+        else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) x[i] = w[i];
+        }
+        __builtin_nontemporal_store(x, (words *)p);
+    }
+}
+
 // Elements one access may take when every row starts at `stride` elements behind the one before: the largest power of two
 // that divides the row length, every stride and every pointer, at most 16 bytes.
 static inline int vec_elems(int elem_size, int64_t row, int64_t stride_a, int64_t stride_b, const void *a, const void *b)

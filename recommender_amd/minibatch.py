@@ -219,8 +219,9 @@ class _Set:
         except (KeyError, AttributeError):
             raise TypeError(f"{name} must be float32 or bfloat16 tensors") from None
         self.sizes = array("q", [t.numel() for t in self.tensors])
-        for t in self.tensors:
-            if not t.is_contiguous() and t.numel() and not _dense(t):
+        self.odd = [i for i, t in enumerate(self.tensors) if not t.is_contiguous()]
+        for i in self.odd:
+            if self.sizes[i] and not _dense(self.tensors[i]):
                 raise ValueError(f"{name} must be dense tensors (no gaps, no element twice)")
         self.addresses = array("Q", [t.data_ptr() for t in self.tensors])
         self.n = len(self.tensors)
@@ -243,15 +244,16 @@ def grad_norm(tensors):
 
 def clip_grads(tensors, max_norm, out=None):
     """Scales all tensors by min(1, max_norm / norm), norm being their global norm, in place or into `out` (tensors of the same
-    shapes, types and strides).  Returns the norm before clipping, without waiting for it."""
+    sizes and types, in the same order of elements).  Returns the norm before clipping, without waiting for it."""
     grads = _Set(tensors, "tensors")
     if not max_norm > 0:
         raise ValueError("max_norm must be positive")
     to = grads
     if out is not None:
         to = _Set(out, "out")
-        if to.n != grads.n or to.dtypes != grads.dtypes or any(
-                o.shape != t.shape or o.stride() != t.stride() for o, t in zip(to.tensors, grads.tensors)):
+        if to.dtypes != grads.dtypes or to.sizes != grads.sizes or any(
+                to.tensors[i].shape != grads.tensors[i].shape or to.tensors[i].stride() != grads.tensors[i].stride()
+                for i in grads.odd + to.odd):
             raise ValueError("out must have a tensor like each of tensors")
     with _On(*grads.tensors, *(to.tensors if to is not grads else ())) as on:
         norm = torch.empty((), dtype=torch.float32, device=on.device)
