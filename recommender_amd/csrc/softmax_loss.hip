@@ -443,16 +443,38 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                             for (int i = 0; i < 4; ++i) e[4 * j + i] *= v[i];
                         }
                     }
-                    if (hits) {             // the target: -g (1 - p_t) in the place of g p_t
+                    // Rows whose target is one of these items: -g (1 - p_t) in the place of g p_t.  It outweighs all else in an
+                    // item's gradient, so bf16 rows do not leave it to the matrix product, which would round it to 8 bits (the
+                    // error of a weighted batch's dW rose by half): it is added to the item's sums in fp32, row by row - one
+                    // row in n_items / 32 tiles.
+                    if (hits) {
                         uint32_t mine = 0;  // rows of the 32 whose target is this lane's item
                         for (uint32_t h = hits; h; h &= h - 1) {
                             const int r = __builtin_ctz(h);
-                            mine |= (uint32_t)(__builtin_amdgcn_readlane((int)at, r) == 32 * u + col) << r;
+                            const bool own = __builtin_amdgcn_readlane((int)at, r) == 32 * u + col;
+                            mine |= (uint32_t)own << r;
+                            if constexpr (PL == 1) {
+                                const int row = sub * 32 + r, sw = swizzle<CH>(row);
+                                const float q = own ? -l_q[buf * TB + row] : 0.f;
+                                sum[u] += kh ? 0.f : q;
+#pragma unroll
+                                for (int c = 0; c < 4 * DT; ++c) {
+                                    const uint2 x = *(const uint2 *)(lds + buf * BUF + row * DP * 2 + (c ^ sw) * 16 + kh * 8);
+                                    f32x16 &v = o[u][c / 4];
+                                    const int j = c % 4 * 4;
+                                    v[j] = fmaf(q, bf16_lo(x.x), v[j]);
+                                    v[j + 1] = fmaf(q, bf16_hi(x.x), v[j + 1]);
+                                    v[j + 2] = fmaf(q, bf16_lo(x.y), v[j + 2]);
+                                    v[j + 3] = fmaf(q, bf16_hi(x.y), v[j + 3]);
+                                    __builtin_amdgcn_sched_barrier(0);
+                                }
+                            }
                         }
                         mine >>= 4 * kh;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (4 * TB + sub * 32 + 8 * j) * 4);
+                            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                            if constexpr (PL == 3) v = *(const LDS_AS f32x4 *)(l3 + at_i + (4 * TB + sub * 32 + 8 * j) * 4);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) e[4 * j + i] = (mine >> (8 * j + i)) & 1 ? -v[i] : e[4 * j + i];
                         }
