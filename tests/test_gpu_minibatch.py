@@ -188,7 +188,9 @@ def loss_tolerances(out, mass, n, items, d, dtype):
 
 
 LOSS_CASES = [(1, 1, 1), (1, 5, 8), (3, 31, 40), (33, 64, 16), (40, 33, 32), (64, 1000, 64), (129, 257, 100), (200, 700, 128),
-              (31, 2000, 129), (65, 300, 192), (130, 500, 193), (300, 129, 256), (1000, 40, 24)]
+              (31, 2000, 129), (65, 300, 192), (130, 500, 193), (300, 129, 256), (1000, 40, 24),
+              # more rows than convert the other side on the way: the planes' kernels, of every width
+              (700, 900, 32), (600, 1100, 64), (513, 257, 65), (530, 2100, 128), (1025, 333, 192), (520, 1500, 256), (1999, 77, 250)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -227,9 +229,10 @@ def test_softmax_loss_many_items_and_rows():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_softmax_loss_masks(dtype):
+@pytest.mark.parametrize("n, d", [(70, 48), (620, 128), (600, 250)])
+def test_softmax_loss_masks(dtype, n, d):
     g = gen(8)
-    n, items, d = 70, 300, 48
+    items = 300
     x, w, t, b = loss_case(g, n, items, d, dtype, True)
     out_of = torch.rand(items, device="cuda", generator=g) < 0.4
     out_of[64:128] = True                                         # a whole tile
@@ -260,6 +263,61 @@ def test_softmax_loss_masks(dtype):
     live = t >= 0
     assert bool((loss[live] == math.inf).all()) and bool((lse[live] == -math.inf).all())
     assert float(dx.abs().sum()) == 0 and float(dw.abs().sum()) == 0 and float(db.abs().sum()) == 0
+
+
+def test_softmax_loss_first_items_masked():
+    """No item of the catalogue among the first ones: the sums' reference is set late, and far from the masked zeros."""
+    n, items, d = 40, 400, 32
+    g = gen(81)
+    for shift in (-300.0, 300.0):                                 # e^z is far outside fp32
+        x, w, t, b = loss_case(g, n, items, d, F32, True)
+        b += shift
+        b[:200] = -math.inf
+        t = 200 + t % 200
+        out, mass = loss_want(x, w, t, b, 1.0)
+        tol = loss_tolerances(out, mass, n, items, d, F32)
+        got = ra.softmax_loss_grads(x, w, t, bias=b)
+        for k in range(5):
+            close(got[k], out[k], tol[k])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_softmax_loss_targets_keep_their_digits(dtype):
+    """Weights that are no powers of two: the target's -g (1 - p) outweighs all else in an item's gradient.  In bf16 it enters in
+    fp32, the other items' g p rounded to 8 bits, so a row of dW is off by its own rounding and by those of the others' only."""
+    g = gen(82)
+    for n, items, d in ((37, 500, 40), (600, 2000, 128)):
+        x, w, t, b = loss_case(g, n, items, d, dtype, True)
+        each = torch.rand(n, device="cuda", generator=g) + 0.1
+        out, _ = loss_want(x, w, t, b, 1.0, each)
+        z = torch.softmax(x.double() @ w.double().T + b.double(), 1)
+        others = (z * (torch.arange(items, device="cuda")[None, :] != t[:, None].long()) * each.double()[:, None]).T @ x.double().abs()
+        _, _, _, dw, _ = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+        held = 2.0 ** -8 if dtype == BF16 else 4 * U
+        # the logits' errors move all of a row's terms: 30 is above every |z|, |x| |w| sum and term count in use here
+        room = (d + items / 32 + n + 200) * U * 30 * (each.double()[None, :] @ x.double().abs())
+        close(dw, out[3], half(dtype) * out[3].abs() + held * others + room + TINY)
+
+
+def test_softmax_loss_many_wide_items():
+    """A table of more than 2^32 bytes and 2^31 elements: every item but three is zero, so the sums are known."""
+    items, d = (1 << 23) + 77, 256
+    table = torch.zeros(items, d, dtype=BF16, device="cuda")
+    for k, v in enumerate((5, items - 1, items - 70)):
+        table[v, k] = 4.0
+    x = torch.zeros(3, d, dtype=BF16, device="cuda")
+    x[0, 0], x[1, 1], x[2, 2] = 1.0, 2.0, 4.0                     # logits 4, 8 and 16 on an item each
+    t = torch.tensor([5, items - 1, 9], dtype=torch.int32, device="cuda")
+    loss, lse, dx, dw, _ = ra.softmax_loss_grads(x, table, t)
+    top = torch.tensor([4.0, 8.0, 16.0], dtype=torch.float64)
+    want = torch.log(items - 1 + torch.exp(top))
+    # a lane adds some 10^6 ones and half a chip's lanes join: 2^-24 of the sum a step, far from its own share of them
+    assert (lse.double().cpu() - want).abs().max() < 1e-3
+    assert (loss.double().cpu() - (want - torch.tensor([4.0, 8.0, 0.0], dtype=torch.float64))).abs().max() < 1e-3
+    p = torch.exp(top - want)
+    assert abs(float(dx[0, 0]) - 4 * (float(p[0]) - 1)) < 0.02 and abs(float(dx[2, 2]) - 4 * float(p[2])) < 0.02
+    assert abs(float(dw[items - 1, 1]) - 2 * (float(p[1]) - 1)) < 0.02 and abs(float(dw[items - 70, 2]) - 4 * float(p[2])) < 0.02
+    assert abs(float(dw[9, 2]) + 4) < 0.02 and float(dw[items - 2].abs().sum()) < 1e-4
 
 
 def test_softmax_loss_not_a_number_shows():
@@ -435,6 +493,21 @@ def test_ranking_step():
     close(loss, want[0], 1e-5 + torch.zeros_like(want[0]))
     for got, x in ((P, want[2]), (Q, want[3]), (b, want[4])):
         close(got, x, 2 * U * x.abs() + 0.5 * 0.05 * 1e-5)
+
+
+def test_ranking_step_bf16_without_bias_or_clipping():
+    g = gen(38)
+    P, Q = normal(g, 50, 64, dtype=BF16), normal(g, 300, 64, dtype=BF16)
+    u, i = ids_of(g, 200, 50), ids_of(g, 200, 300)
+    u[7], i[7] = -1, -1                                           # a padding row
+    before = [P.clone(), Q.clone()]
+    x = ra.embedding(P, u)
+    loss, _, dx, dq, _ = ra.softmax_loss_grads(x, Q, i, scale=0.2, weights=1.0 / 200)
+    dp = ra.embedding_grad(dx, u, 50)
+    got, norm = ra.ExplicitMF.ranking_step(u, i, P, Q, lr=3.0, scale=0.2)
+    assert torch.equal(got, loss) and torch.equal(norm, ra.grad_norm([dp, dq]))
+    for t, b, d in ((P, before[0], dp), (Q, before[1], dq)):
+        assert torch.equal(t, b.sub(d, alpha=3.0))
 
 
 def test_captured_step_replays():
