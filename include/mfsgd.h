@@ -310,9 +310,9 @@ int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_
 /* Softmax cross entropy of x [n][d] against the items' table [n_items][d], 1 <= d <= 256, without keeping the n x n_items
  * logits z_rv = scale * x_r . table_v + bias_v (bias may be NULL):
  *   lse[r] = log sum_v exp z_rv,   loss[r] = lse[r] - z_{r, targets[r]}.
- * A bias of -inf (or below -2e38) takes an item out of the catalogue; a row whose target is out has the loss +inf, with
- * every item out also the lse -inf and no gradient.  A padding row's x is not looked at: loss and lse are 0.
- * scale > 0. */
+ * A bias of -inf takes an item out of the catalogue, whatever its row holds; a row whose target is out has the loss +inf and
+ * no gradient, with every item out also the lse -inf.  A padding row's x is not looked at: loss and lse are 0.
+ * 0 < scale <= 1e20, and bias / scale and bias * log2(e) have to be finite in float32 (or the bias -inf). */
 int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads);
 int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets,
                            const float *bias, int64_t n, int64_t n_items, int32_t d, float scale, int32_t dtype,
@@ -332,7 +332,7 @@ int64_t mfsgd_grad_norm_workspace(const int64_t *h_sizes, int32_t n_tensors);
 int mfsgd_hip_grad_norm(const void *const *h_grads, const int64_t *h_sizes, const int32_t *h_dtypes, int32_t n_tensors,
                         float *norm, void *workspace, int64_t workspace_bytes, void *stream);
 /* h_out[i] = h_grads[i] * min(1, max_norm / norm); h_out NULL, or h_out[i] == h_grads[i]: in place, and then nothing is
- * written where norm <= max_norm.  max_norm > 0.  A norm that is not a number makes every gradient not a number, an
+ * written where norm <= max_norm.  No two tensors of a call may share memory.  max_norm > 0.  A norm that is not a number makes every gradient not a number, an
  * infinite one makes the finite gradients zero. */
 int mfsgd_hip_clip_grads(const void *const *h_grads, void *const *h_out, const int64_t *h_sizes, const int32_t *h_dtypes,
                          int32_t n_tensors, float max_norm, float *norm, void *workspace, int64_t workspace_bytes,

@@ -53,6 +53,7 @@ struct StreamArgs {
     const __bf16 *sm_planes;            // else: planes of the streamed rows, DP wide, zero padded
     int64_t planes_stride, plane;
     int32_t d, n_items;
+    int32_t clear;                      // pass 1: sm_planes is the table itself, and items may be out of the catalogue
     const int32_t *targets;             // of the x rows
     const float *bias;                  // of the items, may be NULL
     float c, inv_scale;                 // scale log2(e), 1 / scale
@@ -197,8 +198,9 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     for (int u = 0; u < UT; ++u) {
         const int32_t row = std::min(st0 + 32 * u + col, n_st - 1);
         target[u] = MODE == TABLE ? 0 : a.targets[row];
-        const bool live = MODE == TABLE || (uint32_t)target[u] < (uint32_t)a.n_items;        // padding is not looked at
         b2[u] = (MODE == TABLE && a.bias) ? a.bias[row] * LOG2E : 0.f;
+        // neither padding nor an item that is out of the catalogue is looked at
+        const bool live = MODE == TABLE ? b2[u] != -INFINITY : (uint32_t)target[u] < (uint32_t)a.n_items;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             Piece<T> raw;
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             for (int q = 0; q < HOLD; ++q) {
                 const int slot = q * 256 + tid, r = slot / CH, c = (slot % CH) ^ swizzle<CH>(slot / CH);
                 const int32_t row = t * TB + std::min(r, last);
-                const bool live = MODE != TABLE || (uint32_t)a.targets[row] < (uint32_t)a.n_items;
+                const bool live = MODE == TABLE ? (uint32_t)a.targets[row] < (uint32_t)a.n_items : !a.bias || a.bias[row] != -INFINITY;
                 held |= (uint32_t)live << q;
                 load_piece((const T *)a.sm.p + row * a.sm.stride, c * 8, a.d, a.sm.vec, hold[q]);
             }
@@ -280,6 +282,18 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
         } else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        if constexpr (MODE != TABLE && !CONV && PL == 1) {
+            if (a.clear) {                              // rows of items that are out: whatever they hold, zero from here on
+                const uint64_t out = __ballot(lane < TB && l_init[buf * TB + lane % TB] == -INFINITY);
+                if (out) {                              // the same in all four waves
+                    for (uint64_t h = out; h; h &= h - 1) {
+                        const int r = __builtin_ctzll(h);
+                        if ((r & 3) == wave && lane < CH) *(uint4 *)(lds + buf * BUF + r * DP * 2 + lane * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncthreads();
+                }
+            }
+        }
     };
 
     f32x16 o[UT][MODE == LOSS ? 1 : DT];
@@ -580,17 +594,18 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     }
 }
 
-// rows -> planes of bf16, dp wide, columns from d on zero; with targets: the rows that take no part are zero
+// rows -> planes of bf16, dp wide, columns from d on zero; the x rows that take no part (targets) and the items that are out of
+// the catalogue (bias) are zero, whatever they hold
 template <typename T, int PL>
 __global__ __launch_bounds__(256) void k_planes(const Rows src, int32_t d, int32_t dp, const int32_t *__restrict__ targets, int32_t n_items,
-                                                __bf16 *__restrict__ dst)
+                                                const float *__restrict__ bias, __bf16 *__restrict__ dst)
 {
     const int32_t per = dp / 8;
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (p >= (int64_t)src.n * per) return;
     const int64_t r = p / per;
     const int32_t c = (int32_t)(p - r * per) * 8;
-    const bool live = !targets || (uint32_t)targets[r] < (uint32_t)n_items;
+    const bool live = targets ? (uint32_t)targets[r] < (uint32_t)n_items : !bias || bias[r] != -INFINITY;
     Piece<T> raw;
     bf16x8 v[PL];
     load_piece((const T *)src.p + r * src.stride, c, d, src.vec, raw);
@@ -627,9 +642,13 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
         if (dx) for (int c = lane; c < a.d; c += 64) store_f32(dx + r * a.d + c, 0.f);
         return;
     }
-    float dot = 0.f;
-    for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
-    const float z = (wave_sum(dot) * a.scale + (a.bias ? a.bias[t] : 0.f)) * LOG2E;      // the target's logit, log2
+    const float bias = a.bias ? a.bias[t] : 0.f;
+    float z = -INFINITY;                                       // the target's logit, log2
+    if (bias != -INFINITY) {
+        float dot = 0.f;
+        for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
+        z = (wave_sum(dot) * a.scale + bias) * LOG2E;
+    }
     float m = -INFINITY;
     bool bad = false;
     for (int s = lane; s < a.splits; s += 64) {
@@ -639,7 +658,8 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
     const float top = fmaxf(m, z);
-    const bool none = top == -INFINITY && !(z != z) && !__ballot(bad);       // every item is out of the catalogue
+    const bool none = z == -INFINITY && !__ballot(bad);        // the target, or every item, is out of the catalogue: no gradient
+    const bool empty = none && m == -INFINITY;
     // Everything relative to the target's logit unless it lies so far below that the others' share would overflow: the loss is
     // then log1p(others), with no difference of nearly equal numbers in it
     const bool near = z > m - 64.f;
@@ -652,7 +672,7 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
     const float q = none ? 0.f : others / all;                 // 1 - p_t
     if (lane == 0 && wave == 0) {
         a.loss[r] = loss;
-        a.lse[r] = none ? -INFINITY : log_all + ref * LN2;
+        a.lse[r] = empty ? -INFINITY : log_all + ref * LN2;
     }
     if (!a.row_init) return;
     const float g = a.weights ? a.weights[r] : 1.f;
@@ -835,8 +855,10 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
     if (!p.conv) {
         auto blocks = [&](int64_t rows) { return dim3((unsigned)((rows * (p.dp / 8) + 255) / 256)); };
-        if (grads) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, xr, d, p.dp, targets, (int32_t)n_items, xp);
-        if (!as_is) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, wr, d, p.dp, (const int32_t *)nullptr, 0, wp);
+        if (grads) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, xr, d, p.dp, targets, (int32_t)n_items,
+                                      (const float *)nullptr, xp);
+        if (!as_is) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, wr, d, p.dp, (const int32_t *)nullptr, 0,
+                                        bias, wp);
         MF_LAUNCH_CHECK();
     }
 
@@ -852,6 +874,7 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     a.sm_planes = as_is ? (const __bf16 *)w : wp;
     a.planes_stride = as_is ? ws_ : p.dp;
     a.plane = n_items * p.dp;
+    a.clear = as_is && bias;
     a.splits = p.splits1; a.row_tiles = p.rt1;
     a.part_m = (float *)(ws + p.m1); a.part_s = (float *)(ws + p.s1); a.part_o = (float *)(ws + p.o1);
     if (const int rc = grads ? launch_stream_d<T, LOSS_SUMS>(p.dp, p.conv, a, st) : launch_stream_d<T, LOSS>(p.dp, p.conv, a, st)) return rc;
@@ -897,7 +920,7 @@ int check_loss(const char *who, const void *x, int64_t xs, const void *w, int64_
     MF_ARG(n >= 0 && n <= INT32_MAX / 4 && n_items >= 1 && n_items <= INT32_MAX / 4 && d >= 1 && d <= 256 && xs >= d && ws_ >= d,
            "%s: bad shape (1 <= d <= 256, at least one item, rows and items below 2^29)", who);
     MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "%s: unknown dtype %d", who, dtype);
-    MF_ARG(scale > 0 && scale <= 1e30f, "%s: scale must be positive and finite", who);
+    MF_ARG(scale > 0 && scale <= 1e20f, "%s: scale must be positive and at most 1e20", who);
     if (n == 0 && !grads) return MFSGD_OK;
     MF_ARG(w && (n == 0 || (x && targets && loss && lse)), "%s: null pointer", who);
     const int64_t need = loss_plan(n, n_items, d, dtype, grads).bytes;

@@ -151,16 +151,17 @@ def _loss_args(x, table, targets, bias, scale):
         raise ValueError("softmax_loss: the table has no items")
     if tuple(targets.shape) != (n,):
         raise ValueError("targets must have an element for every row of x")
-    if not 0 < scale <= 1e30:
-        raise ValueError("scale must be positive and finite")
+    if not 0 < scale <= 1e20:
+        raise ValueError("scale must be positive and at most 1e20")
     return x, xs, table, ts, targets, _vector(bias, table.shape[0], "bias")
 
 
 def softmax_loss(x, table, targets, bias=None, scale=1.0):
     """Cross entropy of the softmax over all items: (loss [n], lse [n]) in float32, with the logits
     z = scale * x @ table.T + bias, lse = logsumexp(z), loss = lse - z[targets].  Rows of at most 256 elements.  A padding row
-    (target < 0) has loss and lse 0 and its x is not looked at; a target behind the table gives a loss that is not a number;
-    a bias of -inf takes an item out of the catalogue."""
+    (target < 0) has loss and lse 0 and its x is not looked at; a target behind the table gives a loss that is not a number.  A
+    bias of -inf takes an item out of the catalogue, whatever its row holds; as a target it gives the loss +inf (and no
+    gradient)."""
     x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
     n, d = x.shape
     with _On(x, table, targets, bias) as on:
