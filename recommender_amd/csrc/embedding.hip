@@ -51,9 +51,9 @@ int launch_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d, 
 {
     if (n_rows == 0) { table = out; stride = 0; }       // nothing is taken from it, but the first piece is always asked for
     const int v = vec_elems(sizeof(T), d, stride, d, table, out);
-    // An output larger than the last-level cache goes past the caches, which then hold the table (2 M rows of 512 bytes: 321 ->
-    // 224 us); a smaller one stays for whoever reads it next (1 M rows of 200 bytes: 47 us either way)
-    const int past = n * d * (int64_t)sizeof(T) > ((int64_t)256 << 20);
+    // A large output goes past the caches, which then hold the table: into memory not written lately 1 M rows of 200 bytes take 42
+    // us against 68, 2 M of 512 bytes 224 against 321.  One that fits the L2s twice stays there for whoever reads it next
+    const int past = n * d * (int64_t)sizeof(T) > ((int64_t)64 << 20);
     const unsigned grid = (unsigned)((n * (d / v) + 256 * PIECES - 1) / (256 * PIECES));
 #define MF_EMB(V_) hipLaunchKernelGGL((k_embedding<T, V_>), dim3(grid), dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, past, out)
     if constexpr (sizeof(T) == 2) {
