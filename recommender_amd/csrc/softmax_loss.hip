@@ -189,32 +189,6 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     const int32_t tiles = (n_sm + TB - 1) / TB;
     const int32_t t0 = (int32_t)((int64_t)tiles * split / a.splits), t1 = (int32_t)((int64_t)tiles * (split + 1) / a.splits);
 
-    constexpr int NB = S::NB, KR = KS - NB;
-    bf16x8 b[UT][PL][KR];
-    LDS_AS char *l_b = (LDS_AS char *)lds + 2 * BUF + 2 * TB * 16 + (wave * NB * PL * 64 + lane) * 16;
-    int32_t target[UT];
-    float b2[UT];
-#pragma unroll
-    for (int u = 0; u < UT; ++u) {
-        const int32_t row = std::min(st0 + 32 * u + col, n_st - 1);
-        target[u] = MODE == TABLE ? 0 : a.targets[row];
-        b2[u] = (MODE == TABLE && a.bias) ? a.bias[row] * LOG2E : 0.f;
-        // neither padding nor an item that is out of the catalogue is looked at
-        const bool live = MODE == TABLE ? b2[u] != -INFINITY : (uint32_t)target[u] < (uint32_t)a.n_items;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            Piece<T> raw;
-            bf16x8 v[PL];
-            load_piece((const T *)a.st.p + row * a.st.stride, 16 * s + 8 * kh, a.d, a.st.vec, raw);
-            split_piece(raw, live, v);
-#pragma unroll
-            for (int p = 0; p < PL; ++p) {
-                if (s < KR) b[u][p][s] = v[p];
-                else *(LDS_AS bf16x8 *)(l_b + ((s - KR) * PL + p) * 1024) = v[p];       // read by the same lane only
-            }
-        }
-    }
-
     // A tile goes straight from memory to LDS, 1 KB a wave and instruction; its place is the lane's, so the swizzle is in
     // which piece a lane asks for.  Where few workgroups read the streamed rows (CONV) they take them as they are and
     // convert them on the way, through registers.
@@ -225,8 +199,23 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     for (int v = 0; v < 2; ++v) from[v] = (tid / CH) * (int32_t)a.planes_stride + ((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 8;
     Piece<T> hold[HOLD ? HOLD : 1];
     uint32_t held = 0;                                  // bit q: row of piece q takes part
+    // What goes with a streamed row.  Asked for in front of the tile and put into LDS when the tile is there: to put it there at
+    // once would wait for it, and with it for all that was asked for before.
+    float p_init = 0.f, p_g = 0.f, p_q = 0.f;
+    int32_t p_t = 0;
     auto stage = [&](int32_t t, int buf) {
         const int32_t last = std::min(TB, n_sm - t * TB) - 1;
+        if (tid < TB) {
+            const bool in = tid <= last;
+            const int32_t row = t * TB + std::min(tid, last);
+            if constexpr (MODE == TABLE) {
+                p_init = in ? a.row_init[row] : -INFINITY;
+                if (a.row_g) p_g = a.row_g[row];
+                p_q = a.row_q[row];
+                p_t = in ? a.targets[row] : -1;
+            } else
+                p_init = !in ? -INFINITY : a.bias ? a.bias[row] : 0.f;
+        }
         if constexpr (CONV) {
             held = 0;
 #pragma unroll
@@ -258,17 +247,6 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                 }
             }
         }
-        if (tid < TB) {
-            const bool in = tid <= last;
-            const int32_t row = t * TB + std::min(tid, last);
-            if constexpr (MODE == TABLE) {
-                l_init[buf * TB + tid] = in ? a.row_init[row] : -INFINITY;
-                if (a.row_g) l_g[buf * TB + tid] = a.row_g[row];
-                l_q[buf * TB + tid] = a.row_q[row];
-                l_t[buf * TB + tid] = in ? a.targets[row] : -1;
-            } else
-                l_init[buf * TB + tid] = in ? (a.bias ? a.bias[row] * a.inv_scale : 0.f) : -INFINITY;
-        }
     };
     auto commit = [&](int buf) {                        // what stage() began is in LDS afterwards
         if constexpr (CONV) {
@@ -281,6 +259,14 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             }
         } else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (tid < TB) {
+            l_init[buf * TB + tid] = MODE == TABLE ? p_init : p_init * a.inv_scale;
+            if constexpr (MODE == TABLE) {
+                l_g[buf * TB + tid] = p_g;
+                l_q[buf * TB + tid] = p_q;
+                l_t[buf * TB + tid] = p_t;
+            }
+        }
         __syncthreads();
         if constexpr (MODE != TABLE && !CONV && PL == 1) {
             if (a.clear) {                              // rows of items that are out: whatever they hold, zero from here on
@@ -337,7 +323,34 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
         }
     };
 
-    if (t0 < t1) stage(t0, 0);
+    if (t0 < t1) stage(t0, 0);                          // in flight while the stationary rows are fetched and split
+
+    constexpr int NB = S::NB, KR = KS - NB;
+    bf16x8 b[UT][PL][KR];
+    LDS_AS char *l_b = (LDS_AS char *)lds + 2 * BUF + 2 * TB * 16 + (wave * NB * PL * 64 + lane) * 16;
+    int32_t target[UT];
+    float b2[UT];
+#pragma unroll
+    for (int u = 0; u < UT; ++u) {
+        const int32_t row = std::min(st0 + 32 * u + col, n_st - 1);
+        target[u] = MODE == TABLE ? 0 : a.targets[row];
+        b2[u] = (MODE == TABLE && a.bias) ? a.bias[row] * LOG2E : 0.f;
+        // neither padding nor an item that is out of the catalogue is looked at
+        const bool live = MODE == TABLE ? b2[u] != -INFINITY : (uint32_t)target[u] < (uint32_t)a.n_items;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            Piece<T> raw;
+            bf16x8 v[PL];
+            load_piece((const T *)a.st.p + row * a.st.stride, 16 * s + 8 * kh, a.d, a.st.vec, raw);
+            split_piece(raw, live, v);
+#pragma unroll
+            for (int p = 0; p < PL; ++p) {
+                if (s < KR) b[u][p][s] = v[p];
+                else *(LDS_AS bf16x8 *)(l_b + ((s - KR) * PL + p) * 1024) = v[p];       // read by the same lane only
+            }
+        }
+    }
+
     commit(0);
     for (int32_t t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1;
@@ -755,21 +768,24 @@ PassShape pass_shape(int dp, int mode, bool conv)
     return conv ? pass_shape_d<PL, TABLE, true>(dp) : pass_shape_d<PL, TABLE, false>(dp);
 }
 
-// Parts the streamed axis is cut into: the number with the least time by this reckoning.  A workgroup takes 4 us to start and
-// end; a tile takes what its products take at the chip's measured rate (1000 TFLOP/s), shared by all workgroups at once; a
-// part's sums are written and read again at 4 TB/s; joining a part takes a row's wave a fraction of a wait for memory.
-int parts_of(int64_t n_sm, int64_t n_st, int64_t row_tiles, const PassShape &s, int dp, int products, bool sums)
+// Parts the streamed axis is cut into: the number with the least time by this reckoning.  A workgroup takes 12 us to start and
+// end.  Of a tile it takes alone_us where it has its share of a full CU; with q workgroups a CU that is alone_us sqrt(q^2 + c^2),
+// as measured with one to three of them: fp32 rows (c = 1) keep the matrix cores busy with one, bf16 rows (c = 3), with one
+// product an operand, wait for LDS and memory.  A part's sums are written and read again at 8 TB/s; pass 2 joins its parts in a
+// launch of its own.
+int parts_of(int64_t n_sm, int64_t n_st, int64_t row_tiles, const PassShape &s, int dp, int products, bool sums, bool pass2)
 {
     static const int counts[] = {1, 2, 3, 4, 5, 6, 7, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024};
-    const double tile_us = 2.0 * s.rows * s.tile * dp * products * s.groups * 1e-9;
-    const double part_us = (sums ? n_st * (double)dp * 8 / 4e6 : 0.0) + 0.015;
+    const double alone_us = 2.0 * s.rows * s.tile * dp * products / 4.2e6, c = products >= 6 ? 1.0 : 3.0;
+    const double part_us = (sums ? n_st * (double)dp * 8 / 8e6 : 0.0) + 0.015;
     const int64_t tiles = (n_sm + s.tile - 1) / s.tile;
     int best = 1;
     double least = 1e300;
     for (int k : counts) {
         if (k > tiles) break;
         const double rounds = (double)((row_tiles * k + s.groups - 1) / s.groups);
-        const double us = rounds * ((double)((tiles + k - 1) / k) * tile_us + 4.0) + (k > 1 ? k * part_us : 0.0);
+        const double q = std::min(row_tiles * k / 256.0, s.groups / 256.0);
+        const double us = rounds * ((double)((tiles + k - 1) / k) * alone_us * sqrt(q * q + c * c) + 12.0) + (k > 1 ? k * part_us + 5.0 * pass2 : 0.0);
         if (us < least) { least = us; best = k; }
     }
     return best;
@@ -796,9 +812,9 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     const PassShape s1 = shape(mode1, p.conv), s2 = shape(TABLE, p.conv);
     p.rt1 = (int)((n + s1.rows - 1) / s1.rows);
     const int six = p.planes == 3 ? 6 : 1;
-    p.splits1 = parts_of(n_items, n, p.rt1, s1, p.dp, six * (grads ? 2 : 1), grads);
+    p.splits1 = parts_of(n_items, n, p.rt1, s1, p.dp, six * (grads ? 2 : 1), grads, false);
     p.rt2 = (int)((n_items + s2.rows - 1) / s2.rows);
-    p.splits2 = parts_of(n, n_items, p.rt2, s2, p.dp, six * 2, true);
+    p.splits2 = parts_of(n, n_items, p.rt2, s2, p.dp, six * 2, true, true);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
     if (!p.conv) {
