@@ -25,6 +25,7 @@
 // 2^-9, the outputs' own rounding; fp32 rows: three).
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 #include "rows.h"
 
 namespace {
@@ -194,9 +195,9 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     // convert them on the way, through registers.
     constexpr int STEP = 256 / CH;                      // rows an instruction of the whole workgroup covers
     constexpr bool EVEN = 256 % CH == 0;
-    int32_t from[2];                                    // a lane's offset in the rows of even and odd steps
+    uint32_t from[2];                                   // a lane's byte offset in the rows of even and odd steps
 #pragma unroll
-    for (int v = 0; v < 2; ++v) from[v] = (tid / CH) * (int32_t)a.planes_stride + ((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 8;
+    for (int v = 0; v < 2; ++v) from[v] = (uint32_t)(tid / CH) * (uint32_t)a.planes_stride * 2 + (uint32_t)((tid % CH) ^ swizzle<CH>(tid / CH + v * STEP)) * 16;
     Piece<T> hold[HOLD ? HOLD : 1];
     uint32_t held = 0;                                  // bit q: row of piece q takes part
     // What goes with a streamed row.  Asked for in front of the tile and put into LDS when the tile is there: to put it there at
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                 for (int q = 0; q < Q; ++q) {
                     constexpr int PER = Q / PL;
                     const __bf16 *rows = base + (q / PER) * a.plane + (q % PER) * STEP * a.planes_stride;
-                    __builtin_amdgcn_global_load_lds((const GLB_AS void *)(rows + from[q % PER % 2]),
+                    __builtin_amdgcn_global_load_lds((const GLB_AS void *)((const char *)rows + from[q % PER % 2]),
                                                      (LDS_AS void *)(lds + buf * BUF + (q * 4 + wave) * 1024), 16, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -308,15 +309,15 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             at_t[d][h] = (tr + 8 * h) * DP * 2 + ((4 * d + 2 * half + ((i16 & 3) >> 1)) ^ swizzle<CH>(tr + 8 * h)) * 16 + (i16 & 1) * 8;
 
     // operands: 16 columns of 32 streamed rows for the logits, 32 columns of 16 streamed rows, transposed, for the sums
-    auto load_a = [&](int sub, int s, bf16x8 (&x)[PL]) {
+    auto load_a = [&](int buf, int sub, int s, bf16x8 (&x)[PL]) {
 #pragma unroll
-        for (int p = 0; p < PL; ++p) x[p] = *(const LDS_AS bf16x8 *)(l3 + at_a[s % NA] + (sub * 32 * DP * 2 + p * PLANE + s / NA * NA * 32));
+        for (int p = 0; p < PL; ++p) x[p] = *(const LDS_AS bf16x8 *)(l3 + at_a[s % NA] + (buf * BUF + sub * 32 * DP * 2 + p * PLANE + s / NA * NA * 32));
     };
-    auto load_t = [&](int sub, int n, bf16x8 (&x)[PL]) {
+    auto load_t = [&](int buf, int sub, int n, bf16x8 (&x)[PL]) {
         const int k = n / DT, dt = n % DT;
 #pragma unroll
         for (int p = 0; p < PL; ++p) {
-            const int imm = (sub * 32 + 16 * k) * DP * 2 + p * PLANE + dt / NT * NT * 64;
+            const int imm = buf * BUF + (sub * 32 + 16 * k) * DP * 2 + p * PLANE + dt / NT * NT * 64;
             const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][0] + imm));
             const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4 *)(l3 + at_t[dt % NT][1] + imm));
             x[p] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
@@ -352,8 +353,9 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     }
 
     commit(0);
-    for (int32_t t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
+    // one tile; which of the two places in LDS it has is known at compile time, so that every address is a register and a constant
+    auto walk = [&](int32_t t, auto place) __attribute__((always_inline)) {
+        constexpr int buf = decltype(place)::value;
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
         bool hit_tile = false;                          // does any row's target lie in this tile?
         if constexpr (MODE != TABLE) {
@@ -367,7 +369,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             f32x16 acc[UT];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (sub * 32 + 8 * j) * 4);
+                const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (buf * TB + sub * 32 + 8 * j) * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[0][4 * j + i] = v[i];
             }
@@ -378,14 +380,14 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             // operands are read one group ahead of the products that take them
             bf16x8 x[2][GA][PL];
 #pragma unroll
-            for (int q = 0; q < GA; ++q) load_a(sub, q, x[0][q]);
+            for (int q = 0; q < GA; ++q) load_a(buf, sub, q, x[0][q]);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 if (s % GA == 0) {
                     if (s) __builtin_amdgcn_sched_barrier(0);
                     if (s + GA < KS) {
 #pragma unroll
-                        for (int q = 0; q < GA; ++q) load_a(sub, s + GA + q, x[(s / GA + 1) & 1][q]);
+                        for (int q = 0; q < GA; ++q) load_a(buf, sub, s + GA + q, x[(s / GA + 1) & 1][q]);
                     }
                 }
                 const bf16x8 (&y)[PL] = x[(s / GA) & 1][s % GA];
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             if constexpr (MODE != LOSS) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int q = 0; q < GA; ++q) load_t(sub, q, x[0][q]);
+                for (int q = 0; q < GA; ++q) load_t(buf, sub, q, x[0][q]);
             }
             __builtin_amdgcn_s_setprio(0);
             bf16x8 w[UT][2][PL];       // the exponentials as operands: j 0..7 and 8..15
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                     if (a.row_g) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + (2 * TB + sub * 32 + 8 * j) * 4);
+                            const f32x4 v = *(const LDS_AS f32x4 *)(l3 + at_i + ((2 + buf) * TB + sub * 32 + 8 * j) * 4);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) e[4 * j + i] *= v[i];
                         }
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                            if constexpr (PL == 3) v = *(const LDS_AS f32x4 *)(l3 + at_i + (4 * TB + sub * 32 + 8 * j) * 4);
+                            if constexpr (PL == 3) v = *(const LDS_AS f32x4 *)(l3 + at_i + ((4 + buf) * TB + sub * 32 + 8 * j) * 4);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) e[4 * j + i] = (mine >> (8 * j + i)) & 1 ? -v[i] : e[4 * j + i];
                         }
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                         if (n) __builtin_amdgcn_sched_barrier(0);
                         if (n + GA < 2 * DT) {
 #pragma unroll
-                            for (int q = 0; q < GA; ++q) load_t(sub, n + GA + q, x[(n / GA + 1) & 1][q]);
+                            for (int q = 0; q < GA; ++q) load_t(buf, sub, n + GA + q, x[(n / GA + 1) & 1][q]);
                         }
                     }
                     const bf16x8 (&y)[PL] = x[(n / GA) & 1][n % GA];
@@ -555,13 +557,11 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                 }
             }
         }
-        const uint32_t by = buf ? -BUF : BUF;
-#pragma unroll
-        for (int s = 0; s < NA; ++s) at_a[s] += by;
-#pragma unroll
-        for (int d = 0; d < NT; ++d) { at_t[d][0] += by; at_t[d][1] += by; }
-        at_i += buf ? -TB * 4 : TB * 4;
         commit(buf ^ 1);
+    };
+    for (int32_t t = t0; t < t1; t += 2) {
+        walk(t, std::integral_constant<int, 0>());
+        if (t + 1 < t1) walk(t + 1, std::integral_constant<int, 1>());
     }
 
 #pragma unroll
