@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void k_embedding(const T *table, int64_t strid
 {
     constexpr int U = PIECES;
     const int32_t per = d / V;
-    const int64_t p0 = (int64_t)blockIdx.x * (256 * U), t0 = p0 / per;          // the same for all threads
+    const int64_t p0 = group_id() * (256 * U), t0 = p0 / per;          // the same for all threads
     const int32_t skip = (int32_t)(p0 - t0 * per);
     int32_t id[U], c[U];
 #pragma unroll
@@ -54,8 +54,8 @@ int launch_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d, 
     // A large output goes past the caches, which then hold the table: into memory not written lately 1 M rows of 200 bytes take 42
     // us against 68, 2 M of 512 bytes 224 against 321.  One that fits the L2s twice stays there for whoever reads it next
     const int past = n * d * (int64_t)sizeof(T) > ((int64_t)64 << 20);
-    const unsigned grid = (unsigned)((n * (d / v) + 256 * PIECES - 1) / (256 * PIECES));
-#define MF_EMB(V_) hipLaunchKernelGGL((k_embedding<T, V_>), dim3(grid), dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, past, out)
+    const dim3 grid = grid_of((n * (d / v) + 256 * PIECES - 1) / (256 * PIECES));
+#define MF_EMB(V_) hipLaunchKernelGGL((k_embedding<T, V_>), grid, dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, past, out)
     if constexpr (sizeof(T) == 2) {
         if (v == 8) { MF_EMB(8); MF_LAUNCH_CHECK(); return MFSGD_OK; }
     }
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad,
                                                      int64_t n_rows, int32_t d, const int32_t *__restrict__ first, int hs, float *__restrict__ parts)
 {
     const int gl = threadIdx.x % L;
-    const int32_t chunk = (int32_t)((int64_t)blockIdx.x * (256 / L) + threadIdx.x / L);
+    const int32_t chunk = (int32_t)(group_id() * (256 / L) + threadIdx.x / L);
     const int64_t lo = (int64_t)chunk << hs;
     if (lo >= n) return;
     const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + (1 << hs));
@@ -373,8 +373,9 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
 #pragma unroll
         for (int q = 0; q < V; ++q) acc[q] = 0.f;
     };
-    if ((int)blockIdx.x < joins) {
-        const int64_t a = ((int64_t)blockIdx.x * (256 / L) + threadIdx.x / L) << hs;
+    const int64_t group = group_id();
+    if (group < joins) {
+        const int64_t a = (group * (256 / L) + threadIdx.x / L) << hs;
         if (a >= n) return;
         const uint32_t v = sorted[std::min<int64_t>(n, a + (1 << hs)) - 1].x;
         if (v >= (uint64_t)n_rows) return;
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
         }
         return;
     }
-    const int64_t v0 = ((int64_t)(blockIdx.x - joins) * (256 / L) + threadIdx.x / L) * R;
+    const int64_t v0 = ((group - joins) * (256 / L) + threadIdx.x / L) * R;
     if (v0 >= n_rows) return;
     const int rows = (int)std::min<int64_t>(R, n_rows - v0);
     const int64_t vf = v0 + std::min(gl, rows);
@@ -500,14 +501,14 @@ int launch_sums(const SumArgs<T> &a, hipStream_t st)
     if (a.n > 1 << a.hs) {
         const int64_t chunks = ((int64_t)a.n + (1 << a.hs) - 1) >> a.hs;
         joins = (int)((chunks + G - 1) / G);
-        hipLaunchKernelGGL((k_heavy_parts<T, V, L>), dim3((unsigned)joins), dim3(256), 0, st, a.grad, a.stride, a.sorted, a.n,
+        hipLaunchKernelGGL((k_heavy_parts<T, V, L>), grid_of(joins), dim3(256), 0, st, a.grad, a.stride, a.sorted, a.n,
                            a.n_rows, a.d, a.first, a.hs, a.parts);
         if (a.n > SUPER << a.hs)
             hipLaunchKernelGGL(k_super_parts, dim3((unsigned)((chunks + SUPER - 1) / SUPER)), dim3(256), 0, st, a.sorted, a.n, a.n_rows, a.d,
                                a.first, a.hs, (const float *)a.parts, a.supers);
     }
     constexpr int R = 4, per_group = G * R;           // rows a group (131072 tokens, 59047 rows: 66 us with 2 or 4, 74 with 8), rows a workgroup
-    hipLaunchKernelGGL((k_row_sums<T, V, L, R>), dim3((unsigned)(joins + (a.n_rows + per_group - 1) / per_group)), dim3(256), 0, st, a.grad,
+    hipLaunchKernelGGL((k_row_sums<T, V, L, R>), grid_of(joins + (a.n_rows + per_group - 1) / per_group), dim3(256), 0, st, a.grad,
                        a.stride, a.sorted, a.n, a.n_rows, a.d, a.scale, a.first, a.hs, joins, (const float *)a.parts, (const float *)a.supers, a.accumulate, a.out,
                        a.out_stride);
     MF_LAUNCH_CHECK();

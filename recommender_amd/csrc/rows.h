@@ -94,3 +94,12 @@ static inline int vec_elems(int elem_size, int64_t row, int64_t stride_a, int64_
     return v;
 }
 static inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+// A dimension of a grid holds fewer than 2^32 threads: workgroups from 2^22 on go on in the second dimension.  The last ones may
+// be more than were asked for; every kernel launched like this looks at its own number.
+static inline dim3 grid_of(int64_t groups)
+{
+    const int64_t x = (int64_t)1 << 22;
+    return groups <= x ? dim3((unsigned)groups) : dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+}
+__device__ __forceinline__ int64_t group_id() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }

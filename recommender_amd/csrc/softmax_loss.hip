@@ -614,7 +614,7 @@ __global__ __launch_bounds__(256) void k_planes(const Rows src, int32_t d, int32
                                                 const float *__restrict__ bias, __bf16 *__restrict__ dst)
 {
     const int32_t per = dp / 8;
-    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t p = group_id() * 256 + threadIdx.x;
     if (p >= (int64_t)src.n * per) return;
     const int64_t r = p / per;
     const int32_t c = (int32_t)(p - r * per) * 8;
@@ -642,7 +642,8 @@ template <typename T, int W>
 __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T *__restrict__ x, const T *__restrict__ w, T *__restrict__ dx)
 {
     __shared__ float sums[W][256];
-    const int64_t r = blockIdx.x;
+    const int64_t r = group_id();
+    if (r >= a.n) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int32_t t = a.targets[r];
     const bool in = (uint32_t)t < (uint64_t)a.n_items;
@@ -734,7 +735,7 @@ __global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ pa
                                                     float *__restrict__ db)
 {
     const int32_t per = (d + 3) / 4;
-    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t p = group_id() * 256 + threadIdx.x;
     if (p >= n_items * per) return;
     const int64_t v = p / per;
     const int32_t c = (int32_t)(p - v * per) * 4;
@@ -870,7 +871,7 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     const bool as_is = PL == 1 && d == p.dp && wr.vec == 8 && ws_ < (1 << 20);
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
     if (!p.conv) {
-        auto blocks = [&](int64_t rows) { return dim3((unsigned)((rows * (p.dp / 8) + 255) / 256)); };
+        auto blocks = [&](int64_t rows) { return grid_of((rows * (p.dp / 8) + 255) / 256); };
         if (grads) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, xr, d, p.dp, targets, (int32_t)n_items,
                                       (const float *)nullptr, xp);
         if (!as_is) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, wr, d, p.dp, (const int32_t *)nullptr, 0,
@@ -904,8 +905,8 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
         j.row_g = weights ? (float *)(ws + p.g) : nullptr;
     }
     // four waves a row: 192 parts of one row 12 -> 5 us; one wave where the rows fill the chip
-    if (grads && p.splits1 >= 32) hipLaunchKernelGGL((k_join_rows<T, 4>), dim3((unsigned)n), dim3(256), 0, st, j, x, w, dx);
-    else hipLaunchKernelGGL((k_join_rows<T, 1>), dim3((unsigned)n), dim3(64), 0, st, j, x, w, dx);
+    if (grads && p.splits1 >= 32) hipLaunchKernelGGL((k_join_rows<T, 4>), grid_of(n), dim3(256), 0, st, j, x, w, dx);
+    else hipLaunchKernelGGL((k_join_rows<T, 1>), grid_of(n), dim3(64), 0, st, j, x, w, dx);
     MF_LAUNCH_CHECK();
     if (!grads) return MFSGD_OK;
 
@@ -923,7 +924,7 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     a.out_vec = vec_elems(sizeof(T), d, d, d, dw, dw);
     if (const int rc = launch_stream_d<T, TABLE>(p.dp, p.conv, a, st)) return rc;
     if (p.splits2 > 1) {
-        hipLaunchKernelGGL((k_join_items<T>), dim3((unsigned)((n_items * ((d + 3) / 4) + 255) / 256)), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,
+        hipLaunchKernelGGL((k_join_items<T>), grid_of((n_items * ((d + 3) / 4) + 255) / 256), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,
                            d, p.dp, scale * weight, weight, dw, db);
         MF_LAUNCH_CHECK();
     }
@@ -936,7 +937,7 @@ int check_loss(const char *who, const void *x, int64_t xs, const void *w, int64_
     MF_ARG(n >= 0 && n <= INT32_MAX / 4 && n_items >= 1 && n_items <= INT32_MAX / 4 && d >= 1 && d <= 256 && xs >= d && ws_ >= d,
            "%s: bad shape (1 <= d <= 256, at least one item, rows and items below 2^29)", who);
     MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "%s: unknown dtype %d", who, dtype);
-    MF_ARG(scale > 0 && scale <= 1e20f, "%s: scale must be positive and at most 1e20", who);
+    MF_ARG(scale >= 1e-20f && scale <= 1e20f, "%s: scale must be from 1e-20 to 1e20", who);
     if (n == 0 && !grads) return MFSGD_OK;
     MF_ARG(w && (n == 0 || (x && targets && loss && lse)), "%s: null pointer", who);
     const int64_t need = loss_plan(n, n_items, d, dtype, grads).bytes;

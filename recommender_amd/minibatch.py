@@ -151,8 +151,8 @@ def _loss_args(x, table, targets, bias, scale):
         raise ValueError("softmax_loss: the table has no items")
     if tuple(targets.shape) != (n,):
         raise ValueError("targets must have an element for every row of x")
-    if not 0 < scale <= 1e20:
-        raise ValueError("scale must be positive and at most 1e20")
+    if not 1e-20 <= scale <= 1e20:
+        raise ValueError("scale must be from 1e-20 to 1e20")
     return x, xs, table, ts, targets, _vector(bias, table.shape[0], "bias")
 
 
@@ -161,7 +161,8 @@ def softmax_loss(x, table, targets, bias=None, scale=1.0):
     z = scale * x @ table.T + bias, lse = logsumexp(z), loss = lse - z[targets].  Rows of at most 256 elements.  A padding row
     (target < 0) has loss and lse 0 and its x is not looked at; a target behind the table gives a loss that is not a number.  A
     bias of -inf takes an item out of the catalogue, whatever its row holds; as a target it gives the loss +inf (and no
-    gradient)."""
+    gradient).  float32's lowest value does the same for an item whose row is finite; bias / scale has to stay in float32
+    otherwise.  scale is from 1e-20 to 1e20."""
     x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
     n, d = x.shape
     with _On(x, table, targets, bias) as on:

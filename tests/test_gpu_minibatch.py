@@ -87,6 +87,21 @@ def test_embedding_far_rows():
     assert torch.equal(table[ids.long(), 259].float().cpu(), torch.arange(2.0, 6.0)) and float(table[5].abs().sum()) == 0
 
 
+def test_embedding_many_rows():
+    """More pieces than a dimension of a grid has threads: 2^34 elements come out, the same rows again and again."""
+    d, period = 33, 1 << 10
+    n = (1 << 34) // d + period
+    table = normal(gen(3), 100, d, dtype=BF16)
+    ids = ids_of(gen(4), period, 100).repeat(n // period + 1)[:n]
+    out = ra.embedding(table, ids)
+    whole = n // period * period
+    assert torch.equal(out[:period], table[ids[:period].long()])
+    for a in range(period, whole, 1 << 24):
+        part = out[a:min(a + (1 << 24), whole)].view(-1, period, d)
+        assert bool((part == out[:period]).all())
+    assert torch.equal(out[whole:], out[:n - whole])
+
+
 # ------------------------------------------------------------------ its gradient
 def grad_want(grad, ids, rows, scale):
     inside = (ids >= 0) & (ids < rows)
@@ -130,6 +145,16 @@ def test_embedding_grad(dtype, n, rows, d, kind):
     close(got, full, (count + 1) * U * 1.01 * mass + U * full.abs() + half(dtype) * full.abs() + TINY)
     assert torch.equal(base[:, d:], before[:, d:])                                    # what lies between the rows
     assert torch.equal(base[(count == 0)[:, 0]], before[(count == 0)[:, 0]])
+
+
+def test_embedding_grad_many_table_rows():
+    """More lanes for the table's rows than a dimension of a grid has threads."""
+    rows, d = (1 << 28) + 7, 33
+    ids = torch.tensor([0, rows - 1, 1 << 27, rows - 1, -1, rows - 8], dtype=torch.int32, device="cuda")
+    grad = torch.arange(1.0, 7.0, device="cuda")[:, None].expand(6, d).to(BF16).contiguous()
+    out = ra.embedding_grad(grad, ids, rows)
+    assert out[[0, rows - 1, 1 << 27, rows - 8], d - 1].tolist() == [1.0, 6.0, 3.0, 6.0]
+    assert sum(int((out[a:a + (1 << 24)] != 0).sum()) for a in range(0, rows, 1 << 24)) == 4 * d
 
 
 def test_embedding_grad_is_the_lookups():
@@ -321,6 +346,18 @@ def test_softmax_loss_many_wide_items():
     assert abs(float(dx[0, 0]) - 4 * (float(p[0]) - 1)) < 0.02 and abs(float(dx[2, 2]) - 4 * float(p[2])) < 0.02
     assert abs(float(dw[items - 1, 1]) - 2 * (float(p[1]) - 1)) < 0.02 and abs(float(dw[items - 70, 2]) - 4 * float(p[2])) < 0.02
     assert abs(float(dw[9, 2]) + 4) < 0.02 and float(dw[items - 2].abs().sum()) < 1e-4
+
+
+def test_softmax_loss_many_rows():
+    """More rows than a dimension of a grid has waves."""
+    n = (1 << 26) + 300
+    x, w, t, b = loss_case(gen(84), n, 3, 1, BF16, True)
+    got = ra.softmax_loss(x, w, t, bias=b)
+    for a, z in ((0, 1000), ((1 << 26) - 500, n)):
+        out, mass = loss_want(x[a:z], w, t[a:z], b, 1.0)
+        tol = loss_tolerances(out, mass, z - a, 3, 1, BF16)
+        close(got[0][a:z], out[0], tol[0])
+        close(got[1][a:z], out[1], tol[1])
 
 
 def test_softmax_loss_not_a_number_shows():

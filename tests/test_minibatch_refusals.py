@@ -38,6 +38,7 @@ def _i(*v):
     (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0)), ValueError),
     (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0, 0), scale=0.0), ValueError),
     (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0, 0), scale=float("inf")), ValueError),
+    (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0, 0), scale=1e-21), ValueError),
     (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0, 0), bias=torch.zeros(4)), ValueError),
     (lambda: ra.softmax_loss(_x(), _x(5), _i(0, 0, 0, 0), bias=torch.zeros(5).bfloat16()), ValueError),
     (lambda: ra.softmax_loss_grads(_x(), _x(5), _i(0, 0, 0, 0), weights=torch.zeros(3)), ValueError),
@@ -105,7 +106,7 @@ def test_c_refusals_softmax_loss():
                                                 nbytes, None)
     for kw, word in ((dict(xs=7), "shape"), (dict(ts=7), "shape"), (dict(items=0), "shape"), (dict(d=257, xs=257, ts=257), "shape"),
                      (dict(n=1 << 30), "shape"), (dict(dtype=5), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-                     (dict(scale=float("nan")), "scale"), (dict(ws=None), "workspace"), (dict(ws=p + 8), "workspace"),
+                     (dict(scale=float("nan")), "scale"), (dict(scale=1e-30), "scale"), (dict(ws=None), "workspace"), (dict(ws=p + 8), "workspace"),
                      (dict(nbytes=need - 1), "workspace"), (dict(dx=None), "null"), (dict(dw=None), "null")):
         assert word in _refused(call(**kw)), kw
     assert "null" in _refused(call(n=0, dx=None, dw=None))        # an empty batch still has a table's gradient to write
