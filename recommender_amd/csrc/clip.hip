@@ -13,20 +13,23 @@
 
 namespace {
 
-constexpr int CLIP_MAX = 128;          // tensors a launch: 28 bytes each of the 4 KB of kernel arguments
+// Tensors a launch: 28 bytes each of the 4 KB of kernel arguments.  The host writes all of them for every launch, so a set of a
+// few tensors goes in a short list.
+constexpr int CLIP_MAX = 128, CLIP_FEW = 8;
 constexpr int64_t PIECE_MIN = 4096;    // elements
 constexpr int PIECES = 1024;           // pieces a large set is cut into: four workgroups a CU
 
-struct ClipSet {
-    const void *in[CLIP_MAX];
-    void *out[CLIP_MAX];
-    int64_t size[CLIP_MAX];
-    int32_t first[CLIP_MAX];           // first piece of a tensor, counted from this launch's first; bit 31: bf16
+template <int MAX> struct ClipSet {
+    const void *in[MAX];
+    void *out[MAX];
+    int64_t size[MAX];
+    int32_t first[MAX];                // first piece of a tensor, counted from this launch's first; bit 31: bf16
     int32_t n_tensors;
 };
 
 // piece -> tensor: the last one whose first piece is not behind it (empty tensors have no piece)
-__device__ __forceinline__ int tensor_of(const ClipSet &set, int piece)
+template <int MAX>
+__device__ __forceinline__ int tensor_of(const ClipSet<MAX> &set, int piece)
 {
     int lo = 0, hi = set.n_tensors - 1;
     while (lo < hi) {
@@ -79,7 +82,8 @@ __device__ __forceinline__ double piece_squares(const T *__restrict__ p, int64_t
     return s[0];
 }
 
-__global__ __launch_bounds__(256) void k_squares(const ClipSet set, int64_t piece, double *__restrict__ partial)
+template <int MAX>
+__global__ __launch_bounds__(256) void k_squares(const ClipSet<MAX> set, int64_t piece, double *__restrict__ partial)
 {
     __shared__ double red[4];
     const int t = tensor_of(set, (int)blockIdx.x);
@@ -135,7 +139,8 @@ __device__ __forceinline__ void piece_scale(const T *p, T *o, int64_t n, float f
     }
 }
 
-__global__ __launch_bounds__(256) void k_clip(const ClipSet set, int64_t piece, const double *__restrict__ partial, int32_t n_partial,
+template <int MAX>
+__global__ __launch_bounds__(256) void k_clip(const ClipSet<MAX> set, int64_t piece, const double *__restrict__ partial, int32_t n_partial,
                                               float max_norm, float *__restrict__ norm, int first_launch)
 {
     __shared__ double red[4];
@@ -166,15 +171,15 @@ int64_t piece_count(const int64_t *sizes, int32_t n, int64_t piece)
     return c;
 }
 
-template <typename F>
+template <int MAX, typename F>
 int for_sets(const void *const *in, void *const *out, const int64_t *sizes, const int32_t *dtypes, int32_t n, int64_t piece, F &&launch)
 {
     int64_t before = 0;
     for (int a = 0; a < n;) {
-        ClipSet set;
+        ClipSet<MAX> set;
         int32_t pieces = 0;
         set.n_tensors = 0;
-        for (; a < n && set.n_tensors < CLIP_MAX; ++a) {
+        for (; a < n && set.n_tensors < MAX; ++a) {
             if (sizes[a] == 0) continue;
             const int i = set.n_tensors++;
             set.in[i] = in[a];
@@ -229,10 +234,23 @@ int check_apart(const char *who, const void *const *in, void *const *out, const 
     return MFSGD_OK;
 }
 
+template <int MAX>
 int squares(const void *const *in, const int64_t *sizes, const int32_t *dtypes, int32_t n, int64_t piece, double *partial, hipStream_t st)
 {
-    return for_sets(in, nullptr, sizes, dtypes, n, piece, [&](const ClipSet &set, int32_t pieces, int64_t before) {
-        hipLaunchKernelGGL(k_squares, dim3(pieces), dim3(256), 0, st, set, piece, partial + before);
+    return for_sets<MAX>(in, nullptr, sizes, dtypes, n, piece, [&](const ClipSet<MAX> &set, int32_t pieces, int64_t before) {
+        hipLaunchKernelGGL(k_squares<MAX>, dim3(pieces), dim3(256), 0, st, set, piece, partial + before);
+    });
+}
+
+template <int MAX>
+int clip(const void *const *in, void *const *out, const int64_t *sizes, const int32_t *dtypes, int32_t n, int64_t piece, int32_t pieces,
+         float max_norm, float *norm, double *partial, hipStream_t st)
+{
+    if (const int rc = squares<MAX>(in, sizes, dtypes, n, piece, partial, st)) return rc;
+    int first = 1;
+    return for_sets<MAX>(in, out, sizes, dtypes, n, piece, [&](const ClipSet<MAX> &set, int32_t count, int64_t) {
+        hipLaunchKernelGGL(k_clip<MAX>, dim3(count), dim3(256), 0, st, set, piece, partial, pieces, max_norm, norm, first);
+        first = 0;
     });
 }
 
@@ -253,7 +271,8 @@ int mfsgd_hip_grad_norm(const void *const *h_grads, const int64_t *h_sizes, cons
     if (const int rc = check_set("grad_norm", h_grads, nullptr, h_sizes, h_dtypes, n_tensors, norm, workspace, workspace_bytes)) return rc;
     const int64_t piece = piece_size(h_sizes, n_tensors);
     const int32_t pieces = (int32_t)piece_count(h_sizes, n_tensors, piece);
-    if (const int rc = squares(h_grads, h_sizes, h_dtypes, n_tensors, piece, (double *)workspace, as_stream(stream))) return rc;
+    const auto sum = n_tensors <= CLIP_FEW ? squares<CLIP_FEW> : squares<CLIP_MAX>;
+    if (const int rc = sum(h_grads, h_sizes, h_dtypes, n_tensors, piece, (double *)workspace, as_stream(stream))) return rc;
     hipLaunchKernelGGL(k_norm, dim3(1), dim3(256), 0, as_stream(stream), (const double *)workspace, pieces, norm);
     MF_LAUNCH_CHECK();
     return MFSGD_OK;
@@ -274,12 +293,8 @@ int mfsgd_hip_clip_grads(const void *const *h_grads, void *const *h_out, const i
         MF_LAUNCH_CHECK();
         return MFSGD_OK;
     }
-    if (const int rc = squares(h_grads, h_sizes, h_dtypes, n_tensors, piece, partial, st)) return rc;
-    int first = 1;
-    return for_sets(h_grads, h_out, h_sizes, h_dtypes, n_tensors, piece, [&](const ClipSet &set, int32_t count, int64_t) {
-        hipLaunchKernelGGL(k_clip, dim3(count), dim3(256), 0, st, set, piece, partial, pieces, max_norm, norm, first);
-        first = 0;
-    });
+    const auto run = n_tensors <= CLIP_FEW ? clip<CLIP_FEW> : clip<CLIP_MAX>;
+    return run(h_grads, h_out, h_sizes, h_dtypes, n_tensors, piece, pieces, max_norm, norm, partial, st);
 }
 
 }  // extern "C"

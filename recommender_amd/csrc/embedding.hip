@@ -75,16 +75,21 @@ __device__ __forceinline__ uint32_t sort_key(int32_t id, int64_t n_rows)
 }
 
 // Small batches: the rank of position t is the number of smaller keys plus the number of equal keys in front of it.  16 lanes
-// rank one position, a sixteenth of the keys each, read from LDS four at a time; one launch, no passes.
+// rank one position, a sixteenth of the keys each, read from LDS four at a time; one launch, no passes.  With `first` the groups
+// behind the positions' do the same for the table's rows: first[v] is the number of keys below v, v = 0 .. n_rows.
 constexpr int RANK_MAX = 8192;
-__global__ __launch_bounds__(256) void k_rank(const int32_t *__restrict__ ids, int32_t n, int64_t n_rows, uint2 *__restrict__ sorted)
+__global__ __launch_bounds__(256) void k_rank(const int32_t *__restrict__ ids, int32_t n, int64_t n_rows, uint2 *__restrict__ sorted,
+                                              int32_t *__restrict__ first)
 {
     __shared__ __attribute__((aligned(16))) uint32_t keys[RANK_MAX];
     const int n4 = (n + 3) & ~3, part = threadIdx.x & 15;
     for (int i = threadIdx.x; i < n4; i += 256) keys[i] = i < n ? sort_key(ids[i], n_rows) : 0xffffffffu;
     __syncthreads();
-    const int t = blockIdx.x * 16 + (threadIdx.x >> 4);
-    const uint32_t mine = keys[t < n ? t : 0];
+    const int t_groups = (n + 15) / 16, group = blockIdx.x;
+    const bool of_row = group >= t_groups;
+    const int t = of_row ? -1 : group * 16 + (threadIdx.x >> 4);            // of a row: no equal key counts
+    const int64_t v = (int64_t)(group - t_groups) * 16 + (threadIdx.x >> 4);
+    const uint32_t mine = of_row ? (uint32_t)v : keys[t < n ? t : 0];
     int32_t rank = 0;
     for (int i = 4 * part; i < n4; i += 64) {
         const uint4 k = *(const uint4 *)(keys + i);
@@ -94,7 +99,9 @@ __global__ __launch_bounds__(256) void k_rank(const int32_t *__restrict__ ids, i
     }
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) rank += __shfl_xor(rank, m, 16);
-    if (t < n && part == 0) sorted[rank] = make_uint2(mine, (uint32_t)t);
+    if (part) return;
+    if (of_row) { if (v <= n_rows) first[v] = rank; }
+    else if (t < n) sorted[rank] = make_uint2(mine, (uint32_t)t);
 }
 
 // Large batches: least significant digit first, DIGIT bits a pass, stable.  A tile is SORT_TILE consecutive entries of one
@@ -224,19 +231,14 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint2 *__restrict__ in,
         }
 }
 
-// number of sorted keys below v
-__device__ __forceinline__ int32_t first_of(const uint2 *__restrict__ sorted, int32_t n, uint32_t v)
-{
-    int32_t lo = 0, hi = n;
-    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (sorted[mid].x < v) lo = mid + 1; else hi = mid; }
-    return lo;
-}
-
-// first[v] for v = 0 .. n_rows
+// first[v], the number of sorted keys below v, for v = 0 .. n_rows
 __global__ __launch_bounds__(256) void k_row_first(const uint2 *__restrict__ sorted, int32_t n, int64_t n_rows, int32_t *__restrict__ first)
 {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v <= n_rows) first[v] = first_of(sorted, n, (uint32_t)v);
+    if (v > n_rows) return;
+    int32_t lo = 0, hi = n;
+    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (sorted[mid].x < (uint32_t)v) lo = mid + 1; else hi = mid; }
+    first[v] = lo;
 }
 
 // ------------------------------------------------------------------ sums
@@ -312,7 +314,7 @@ __global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad,
     for (int slot = 0; slot < 2; ++slot) {
         const uint32_t kk = slot ? kl : kf;
         if ((slot && kl == kf) || kk >= (uint64_t)n_rows) continue;
-        const int32_t s = first ? first[kk] : first_of(sorted, n, kk), e = first ? first[kk + 1] : first_of(sorted, n, kk + 1);
+        const int32_t s = first[kk], e = first[kk + 1];
         if (e - s <= 1 << hs) continue;
         for (int32_t c0 = 0; c0 < d; c0 += V * L) {
             const int32_t c = c0 + gl * V;
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(256) void k_super_parts(const uint2 *__restrict__ s
     for (int slot = 0; slot < 2; ++slot) {
         const uint32_t kk = slot ? kl : kf;
         if ((slot && kl == kf) || kk >= (uint64_t)n_rows) continue;
-        const int32_t s = first ? first[kk] : first_of(sorted, n, kk), e = first ? first[kk + 1] : first_of(sorted, n, kk + 1);
+        const int32_t s = first[kk], e = first[kk + 1];
         if (stretches(s, e, hs) <= SUPER) continue;
         for (int32_t c = threadIdx.x; c < d; c += 256) {
             float acc[1] = {};
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
         if (a >= n) return;
         const uint32_t v = sorted[std::min<int64_t>(n, a + (1 << hs)) - 1].x;
         if (v >= (uint64_t)n_rows) return;
-        const int32_t s = first ? first[v] : first_of(sorted, n, v), e = first ? first[v + 1] : first_of(sorted, n, v + 1);
+        const int32_t s = first[v], e = first[v + 1];
         if (e - s <= 1 << hs || s < a) return;
         for (int32_t c = gl * V; c < d; c += V * L) {
             float acc[V] = {};
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
     if (v0 >= n_rows) return;
     const int rows = (int)std::min<int64_t>(R, n_rows - v0);
     const int64_t vf = v0 + std::min(gl, rows);
-    const int32_t f = first ? first[vf] : first_of(sorted, n, (uint32_t)vf);
+    const int32_t f = first[vf];
     const int32_t f_next = __shfl(f, gl < R ? gl + 1 : R, L);
     const int lead = (threadIdx.x & 63) / L * L;         // the group's first lane
     const uint32_t heavy = (uint32_t)(__ballot(gl < rows && f_next - f > 1 << hs) >> lead) & ((1u << R) - 1);
@@ -443,7 +445,6 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
 // what a gradient call keeps in its workspace
 struct GradPlan {
     int passes, bits, per, tiles, hs;
-    bool first_table;
     int64_t sorted[2], counts, totals, first, parts, supers, bytes;
 };
 
@@ -465,9 +466,7 @@ GradPlan grad_plan(int64_t n, int64_t n_rows, int32_t d)
         p.counts = take((int64_t)(1 << p.bits) * p.tiles * 4);
         p.totals = take((int64_t)(1 << p.bits) * 4);
     }
-    // a table of the rows' first places, or (few rows) a search by every group that needs one
-    p.first_table = !small || n_rows > 65536;
-    if (p.first_table) p.first = take((n_rows + 1) * 4);
+    p.first = take((n_rows + 1) * 4);
     // Short stretches keep the wait for a popular row short (131072 tokens of bf16, d = 128: 74 us with 16, 85 with 32, 102
     // with 64), long ones write and read fewer parts (2 M tokens of fp32: 432, 405 and 402 us)
     p.hs = n <= RANK_MAX || n > 256 * 1024 ? 5 : 4;
@@ -532,9 +531,15 @@ int grad_impl(const T *grad, int64_t stride, const int32_t *ids, int64_t n, int6
     const GradPlan p = grad_plan(n, n_rows, d);
     uint2 *sorted[2] = {(uint2 *)(ws + p.sorted[0]), (uint2 *)(ws + p.sorted[1])};
     const int32_t m = (int32_t)n;
+    int32_t *first = (int32_t *)(ws + p.first);
     int at = 0;
+    bool has_first = false;
     if (n <= RANK_MAX) {
-        if (n) hipLaunchKernelGGL(k_rank, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, ids, m, n_rows, sorted[0]);
+        // The rows' first places by ranking while that is less than a launch (32 tokens of a 17770-row table 18.5 -> 14.9 us, 1000
+        // of 1682 rows 19.5 -> 18.0; 8000 of 16000 rows would take 57 instead of 42)
+        has_first = n && n_rows <= 65536 && n * n_rows <= 1 << 25;
+        if (n) hipLaunchKernelGGL(k_rank, dim3((unsigned)((n + 15) / 16 + (has_first ? (n_rows + 16) / 16 : 0))), dim3(256), 0, st, ids, m, n_rows,
+                                  sorted[0], first);
     } else {
         int32_t *counts = (int32_t *)(ws + p.counts), *totals = (int32_t *)(ws + p.totals);
         for (int pass = 0; pass < p.passes; ++pass) {
@@ -551,8 +556,7 @@ int grad_impl(const T *grad, int64_t stride, const int32_t *ids, int64_t n, int6
                                     (const int32_t *)counts, (const int32_t *)totals, sorted[at]);
         }
     }
-    int32_t *first = p.first_table ? (int32_t *)(ws + p.first) : nullptr;
-    if (first)
+    if (!has_first)
         hipLaunchKernelGGL(k_row_first, dim3((unsigned)((n_rows + 256) / 256)), dim3(256), 0, st, (const uint2 *)sorted[at], m, n_rows, first);
     const SumArgs<T> a = {grad, stride, sorted[at], m, n_rows, d, scale, accumulate, first, p.hs, (float *)(ws + p.parts), (float *)(ws + p.supers),
                           out, out_stride};

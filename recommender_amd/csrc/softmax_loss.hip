@@ -187,6 +187,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
     }
     const int32_t n_st = a.st.n, n_sm = a.sm.n;
     const int32_t st0 = (rt * 4 + wave) * (32 * UT);
+    const bool busy = st0 < n_st;
     const int32_t tiles = (n_sm + TB - 1) / TB;
     const int32_t t0 = (int32_t)((int64_t)tiles * split / a.splits), t1 = (int32_t)((int64_t)tiles * (split + 1) / a.splits);
 
@@ -363,6 +364,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
             for (int u = 0; u < UT; ++u) hit_tile |= (uint32_t)(target[u] - t * TB) < (uint32_t)TB;
             hit_tile = __ballot(hit_tile) != 0;
         }
+        if (CONV && !busy) { commit(buf ^ 1); return; }     // all its rows are behind the last one
 #pragma unroll
         for (int sub = 0; sub < TB / 32; ++sub) {
             // logits (in units of scale) of 32 streamed rows: acc[u][j] is row 8 (j / 4) + 4 kh + j % 4 for stationary row `col`
@@ -608,23 +610,30 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 }
 
 // rows -> planes of bf16, dp wide, columns from d on zero; the x rows that take no part (targets) and the items that are out of
-// the catalogue (bias) are zero, whatever they hold
+// the catalogue (bias) are zero, whatever they hold.  Both sides in one launch.
+struct PlaneJob {
+    Rows src;
+    const int32_t *targets;             // of x rows, else NULL
+    const float *bias;                  // of items, may be NULL
+    __bf16 *dst;
+};
 template <typename T, int PL>
-__global__ __launch_bounds__(256) void k_planes(const Rows src, int32_t d, int32_t dp, const int32_t *__restrict__ targets, int32_t n_items,
-                                                const float *__restrict__ bias, __bf16 *__restrict__ dst)
+__global__ __launch_bounds__(256) void k_planes(const PlaneJob x, const PlaneJob w, int64_t x_groups, int32_t n_items, int32_t d, int32_t dp)
 {
-    const int32_t per = dp / 8;
-    const int64_t p = group_id() * 256 + threadIdx.x;
-    if (p >= (int64_t)src.n * per) return;
+    const bool is_x = group_id() < x_groups;
+    const PlaneJob &job = is_x ? x : w;
+    const int32_t per = dp / 8, n = job.src.n;
+    const int64_t p = (group_id() - (is_x ? 0 : x_groups)) * 256 + threadIdx.x;
+    if (p >= (int64_t)n * per) return;
     const int64_t r = p / per;
     const int32_t c = (int32_t)(p - r * per) * 8;
-    const bool live = targets ? (uint32_t)targets[r] < (uint32_t)n_items : !bias || bias[r] != -INFINITY;
+    const bool live = is_x ? (uint32_t)job.targets[r] < (uint32_t)n_items : !job.bias || job.bias[r] != -INFINITY;
     Piece<T> raw;
     bf16x8 v[PL];
-    load_piece((const T *)src.p + r * src.stride, c, d, src.vec, raw);
+    load_piece((const T *)job.src.p + r * job.src.stride, c, d, job.src.vec, raw);
     split_piece(raw, live, v);
 #pragma unroll
-    for (int q = 0; q < PL; ++q) *(bf16x8 *)(dst + (int64_t)q * src.n * dp + r * dp + c) = v[q];
+    for (int q = 0; q < PL; ++q) *(bf16x8 *)(job.dst + (int64_t)q * n * dp + r * dp + c) = v[q];
 }
 
 struct JoinArgs {
@@ -842,7 +851,7 @@ int launch_stream(const StreamArgs &a, hipStream_t st)
     auto kern = k_stream<T, DP, MODE, CONV>;
     constexpr int bytes = Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>::LDS;
     static_assert(bytes <= 160 * 1024, "a CU's LDS");
-    MF_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (bytes > 64 * 1024) MF_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.splits * a.row_tiles)), dim3(256), bytes, st, a);
     MF_LAUNCH_CHECK();
     return MFSGD_OK;
@@ -871,11 +880,10 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     const bool as_is = PL == 1 && d == p.dp && wr.vec == 8 && ws_ < (1 << 20);
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
     if (!p.conv) {
-        auto blocks = [&](int64_t rows) { return grid_of((rows * (p.dp / 8) + 255) / 256); };
-        if (grads) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n), dim3(256), 0, st, xr, d, p.dp, targets, (int32_t)n_items,
-                                      (const float *)nullptr, xp);
-        if (!as_is) hipLaunchKernelGGL((k_planes<T, PL>), blocks(n_items), dim3(256), 0, st, wr, d, p.dp, (const int32_t *)nullptr, 0,
-                                        bias, wp);
+        auto groups = [&](int64_t rows) { return (rows * (p.dp / 8) + 255) / 256; };
+        const PlaneJob jx = {xr, targets, nullptr, xp}, jw = {wr, nullptr, bias, wp};
+        const int64_t gx = grads ? groups(n) : 0, gw = as_is ? 0 : groups(n_items);
+        if (gx + gw) hipLaunchKernelGGL((k_planes<T, PL>), grid_of(gx + gw), dim3(256), 0, st, jx, jw, gx, (int32_t)n_items, d, p.dp);
         MF_LAUNCH_CHECK();
     }
 

@@ -65,7 +65,7 @@ class _On:
         if index != torch.cuda.current_device():
             self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        self.stream = torch.cuda.current_stream(index).cuda_stream
+        self.stream = torch._C._cuda_getCurrentRawStream(index)
         return self
 
     def __exit__(self, *exc):
@@ -172,7 +172,8 @@ def softmax_loss(x, table, targets, bias=None, scale=1.0):
             x.data_ptr(), xs, table.data_ptr(), ts, targets.data_ptr(), None if bias is None else bias.data_ptr(), n,
             table.shape[0], d, scale, _DTYPES[x.dtype], both.data_ptr(), both.data_ptr() + 4 * n, ws.data_ptr(), ws.numel(),
             on.stream))
-    return both[0], both[1]
+    loss, lse = both.unbind()
+    return loss, lse
 
 
 def softmax_loss_grads(x, table, targets, bias=None, scale=1.0, weights=1.0):
@@ -194,7 +195,8 @@ def softmax_loss_grads(x, table, targets, bias=None, scale=1.0, weights=1.0):
             None if each is None else each.data_ptr(), 1.0 if each is not None else float(weights), n, n_items, d, scale,
             _DTYPES[x.dtype], both.data_ptr(), both.data_ptr() + 4 * n, dx.data_ptr(), dtable.data_ptr(),
             None if dbias is None else dbias.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
-    return both[0], both[1], dx, dtable, dbias
+    loss, lse = both.unbind()
+    return loss, lse, dx, dtable, dbias
 
 
 def _dense(t):
