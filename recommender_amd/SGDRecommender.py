@@ -27,7 +27,6 @@ import numpy as np
 
 from . import _abi
 from .numba_methods import mse, mse2, rmse_exact, sgd, sgd2  # noqa: F401  (re-exported like `from numba_methods import *`)
-from .minibatch import clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
 from .Recommender import Recommender
 from .SubSample import SubSample
 
@@ -640,9 +639,14 @@ class ExplicitMF(Recommender):
     def ranking_step(users, items, user_vecs, item_vecs, b_i=None, lr=0.1, max_norm=None, scale=1.0):
         """One minibatch step of the ranking objective that `top_n` answers for: lowers the mean over the batch of
         -log softmax(scale * user_vecs[users] @ item_vecs.T + b_i)[items], in place on the given ROCm tensors (float32 or
-        bfloat16 factors, float32 b_i; users and items int32, an item < 0 is padding).  With `max_norm` the gradients of
-        all factors are clipped to it first.  Returns (loss [n], norm of the gradients); asynchronous, no host copies."""
+        bfloat16 factors, float32 b_i; users and items int32, a user or an item < 0 is padding, one behind its table gives a
+        loss that is not a number and no gradient).  With `max_norm` the gradients of all factors are clipped to it first.
+        Returns (loss [n], norm of the gradients); asynchronous, no host copies."""
+        from .minibatch import clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
+        torch = _abi.torch_mod()
         n = int(users.shape[0])
+        # a row whose user is no row of user_vecs must not reach the items' gradients
+        items = torch.where(users < 0, users, torch.where(users < user_vecs.shape[0], items, 2 ** 31 - 1))
         x = embedding(user_vecs, users)
         loss, _, dx, dq, db = softmax_loss_grads(x, item_vecs, items, bias=b_i, scale=scale, weights=1.0 / max(n, 1))
         dp = embedding_grad(dx, users, user_vecs.shape[0])

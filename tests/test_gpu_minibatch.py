@@ -550,6 +550,19 @@ def test_ranking_step_bf16_without_bias_or_clipping():
         assert torch.equal(t, b.sub(d, alpha=3.0))
 
 
+def test_ranking_step_users_out_of_range():
+    """A user that is no row of the table has no part in the step: padding, or a loss that is not a number."""
+    u, i, P, Q, b = batch(31)
+    far, away = u.clone(), i.clone()
+    far[10], far[11], away[10], away[11] = -1, 90, -1, -1
+    one, two = [t.clone() for t in (P, Q, b)], [P, Q, b]
+    loss, norm = ra.ExplicitMF.ranking_step(far, i, *one, lr=0.5, max_norm=0.05, scale=0.3)
+    want, length = ra.ExplicitMF.ranking_step(u, away, *two, lr=0.5, max_norm=0.05, scale=0.3)
+    assert float(loss[10]) == 0 and math.isnan(float(loss[11])) and torch.equal(norm, length)
+    loss[11] = 0
+    assert torch.equal(loss, want) and all(torch.equal(x, y) for x, y in zip(one, two))
+
+
 def test_captured_step_replays():
     """The whole step in a graph, replayed on new inputs with eager work of the same kind in between."""
     u, i, P, Q, b = batch(31, n=5000)

@@ -1,5 +1,8 @@
 """Calls that the minibatch operators refuse: argument checks come before the device is touched, so they run without a GPU."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -138,3 +141,9 @@ def test_c_refusals_clip():
     sizes = (C.c_int64 * 2)(5, -5)
     assert lib.mfsgd_grad_norm_workspace(sizes, 2) == -1 and lib.mfsgd_grad_norm_workspace(None, 2) == -1
     assert lib.mfsgd_grad_norm_workspace(sizes, 1) > 0
+
+
+def test_the_package_imports_without_torch():
+    code = ("import sys, recommender_amd as ra; assert 'torch' not in sys.modules; ra.embedding; "
+            "assert 'torch' in sys.modules and ra.minibatch.clip_grads is ra.clip_grads and not hasattr(ra, 'nothing')")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
