@@ -332,8 +332,8 @@ int64_t mfsgd_grad_norm_workspace(const int64_t *h_sizes, int32_t n_tensors);
 int mfsgd_hip_grad_norm(const void *const *h_grads, const int64_t *h_sizes, const int32_t *h_dtypes, int32_t n_tensors,
                         float *norm, void *workspace, int64_t workspace_bytes, void *stream);
 /* h_out[i] = h_grads[i] * min(1, max_norm / norm); h_out NULL, or h_out[i] == h_grads[i]: in place, and then nothing is
- * written where norm <= max_norm.  No two tensors of a call may share memory.  max_norm > 0.  A norm that is not a number makes every gradient not a number, an
- * infinite one makes the finite gradients zero. */
+ * written where norm <= max_norm.  No two tensors of a call may share memory.  max_norm > 0.  A norm that is not a number makes
+ * every gradient not a number, an infinite one makes the finite gradients zero. */
 int mfsgd_hip_clip_grads(const void *const *h_grads, void *const *h_out, const int64_t *h_sizes, const int32_t *h_dtypes,
                          int32_t n_tensors, float max_norm, float *norm, void *workspace, int64_t workspace_bytes,
                          void *stream);

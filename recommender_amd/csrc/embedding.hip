@@ -4,7 +4,11 @@
 //
 // The gradient sorts the batch's positions by id (stable: equal ids stay in the order of t), so that a table row's tokens
 // are one stretch of the sorted list; a row is then summed by one group of lanes in fp32, in the order of t, and written
-// once.  No atomics: the same inputs give the same bits.
+// once.  No floating-point atomics: the same inputs give the same bits.
+//
+// 2 M tokens of 512 bytes into 480189 rows: 373 us, of which the sums take 270 (1.28 GB: 4.7 TB/s, a copy reaches 5.1) and the
+// sort and the rows' first places the rest.  131072 bf16 tokens of 256 bytes: 66 us, ten launches of 3 to 20 us that wait for
+// each other; the sums would be 10 us at a copy's rate.  1000 tokens: 17 us, three launches.
 #include <algorithm>
 #include <math.h>
 #include "rows.h"
@@ -13,7 +17,8 @@ namespace {
 
 // ------------------------------------------------------------------ lookup
 // A thread moves PIECES pieces of V elements (one access each), all of them asked for before the first one is used; the pieces
-// of the output are numbered through.
+// of the output are numbered through.  Bound by memory: 1 M bf16 rows of 200 bytes 42 us (5.1 TB/s, what a copy reaches; 96 us
+// with one piece a thread); 32 rows: the launch, 8.4 us from Python.
 constexpr int PIECES = 4;
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d,
@@ -104,9 +109,9 @@ __global__ __launch_bounds__(256) void k_rank(const int32_t *__restrict__ ids, i
     else if (t < n) sorted[rank] = make_uint2(mine, (uint32_t)t);
 }
 
-// Large batches: least significant digit first, DIGIT bits a pass, stable.  A tile is SORT_TILE consecutive entries of one
-// workgroup; a pass counts every tile's digits, turns the counts into first places and moves the entries.
-// An entry is (key, position).
+// Large batches: least significant digit first, up to ten bits a pass, stable.  A tile is 256 PER consecutive entries of one
+// workgroup; a pass counts every tile's digits, turns the counts into first places and moves the entries.  An entry is (key,
+// position).  Bound by latency and LDS atomics, not by the 16 to 32 MB that a pass over 2 M entries moves: 14 + 6 + 23 us.
 constexpr int SORT_BINS = 1024;
 
 template <int PER>

@@ -6,23 +6,35 @@
 //
 // One kernel shape does all the products (k_stream): a wave keeps 32 STATIONARY rows in registers and walks past tiles of
 // STREAMED rows in LDS.  With streamed rows as MFMA rows and stationary rows as MFMA columns a lane ends up with 16 logits
-// of ONE stationary row, so running maximum and sum are private to a lane, and the exponentials are, as they stand, the B
+// of ONE stationary row, so a row's reference and sum are private to two lanes, and the exponentials are, as they stand, the B
 // operand of the second product (the order of the streamed rows inside an operand is free, and the other operand, read
 // transposed from the same LDS tile, takes the same order).
-//   pass 1   stationary x, streamed items:  running maximum, sum and sum_v exp(z - m) w_v, in one walk over the items
-//   combine  joins the parts of the items' axis: lse, loss, dX
-//   pass 2   stationary items, streamed x:  the logits again, now with lse known:  dW, db
+//   planes   rows that are no operands as they are: split, padded, and cleared where they take no part (small batches do
+//            that on the way instead)
+//   pass 1   stationary x, streamed items:  a reference m, sum_v exp(z - m) and sum_v exp(z - m) w_v, in one walk
+//   join     the parts of the items' axis: lse, loss, dX
+//   pass 2   stationary items, streamed x:  the logits again, now with lse known:  dW, db, and a join if x is cut into parts
 // 8 n d V operations, two of the logits, against the 6 that cannot be avoided: keeping the logits would move 2 n V elements
-// to memory and back instead.
+// to memory and back instead (4096 x 624961 in bf16: 10 GB, 2 ms, instead of 1.2 ms of products).
 //
-// The target's own term is left out of pass 1 and added in the combine, in fp32 from the rows themselves: 1 - p_t is then the
-// other items' share, not a difference of rounded numbers, and a well-learnt row's gradient (p_t near 1) keeps its digits.
+// What bounds it: power, then the vector unit.  4096 x 624961 x 256 bf16: 2.23 and 2.43 ms for the passes, 1180 and 1080
+// TFLOP/s; the matrix cores are busy 70 % and 63 % of the cycles at the 1.6 GHz that the card keeps under this load (a library
+// product of 8192 cubed: 1115 TFLOP/s).  8192 x 17770 x 128 fp32: 356 and 402 us, 1260 and 1110 TFLOP/s of bf16 products, busy
+// 80 % and 76 %.  A loss without gradients has an exponential, a multiply-add and an add for 2 d operations: 5003 x 59047 x
+// 100 bf16 97 us, vector unit 60 %, matrix cores 44 %.  LDS: no bank conflicts (swizzle, below), active 30 to 50 %.  A third
+// tile in LDS, so that loads have two tiles' time, changed nothing.  Small problems wait: 12 us a launch to start, fetch and
+// end, which decides the number of parts (parts_of).
+//
+// The target's own term stays out of the matrix products: pass 1 leaves it to the join, which adds it in fp32 from the rows
+// themselves - 1 - p_t is then the other items' share, not a difference of rounded numbers, and a well-learnt row's gradient
+// (p_t near 1) keeps its digits; pass 2 adds a bf16 target's x to its item in fp32.
 //
 // Types: bf16 rows are the operands as they are.  An fp32 row is split into three bf16 rows of 8 bits each (x = x0 + x1 + x2,
 // exact to 2^-24), and a product is the six products of order up to 2 - the three left out are below 2^-24 of it.  Six bf16
 // matrix instructions cost less than one fp32 instruction of the same shape (2.5 PFLOP/s against 157 TFLOP/s).  The
-// exponentials, too, are rounded to bf16 for the second product, as they are written to no memory (bf16 rows: one value of
-// 2^-9, the outputs' own rounding; fp32 rows: three).
+// exponentials, too, are rounded to bf16 for the second product (bf16 rows: once, 2^-9 of a term, what the outputs themselves
+// are rounded by; in three parts it took 30 % more time.  fp32 rows: three parts, exact to 2^-24).  The sum of the
+// exponentials, lse, loss and 1 - p_t are of the unrounded ones.
 #include <algorithm>
 #include <math.h>
 #include <type_traits>
@@ -610,7 +622,8 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
 }
 
 // rows -> planes of bf16, dp wide, columns from d on zero; the x rows that take no part (targets) and the items that are out of
-// the catalogue (bias) are zero, whatever they hold.  Both sides in one launch.
+// the catalogue (bias) are zero, whatever they hold.  Both sides in one launch (1000 x 3706 x 40 step: 49 -> 47 us).  Bound by memory:
+// 59047 rows of 100 bf16, 27 MB: 9 us.
 struct PlaneJob {
     Rows src;
     const int32_t *targets;             // of x rows, else NULL
@@ -645,8 +658,9 @@ struct JoinArgs {
     float *loss, *lse, *row_init, *row_q, *row_g;     // row_init NULL: no gradients
 };
 
-// W waves a row (one, or four where there are many parts): joins the parts of the items' axis, adds the target's own term and writes loss, lse, the row's dX and what
-// pass 2 needs of the row.
+// W waves a row (one, or four where there are many parts): joins the parts of the items' axis, adds the target's own term and
+// writes loss, lse, the row's dX and what pass 2 needs of the row.  Bound by the parts' bytes where there are many rows (4096 rows
+// of 256, 8 parts: 18 us), by a chain of loads where there are few (1000 rows of 40 in 32 parts: 7 us).
 template <typename T, int W>
 __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T *__restrict__ x, const T *__restrict__ w, T *__restrict__ dx)
 {
