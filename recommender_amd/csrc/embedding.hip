@@ -7,7 +7,7 @@
 // once.  No floating-point atomics: the same inputs give the same bits.
 //
 // 2 M tokens of 512 bytes into 480189 rows: 373 us, of which the sums take 270 (1.28 GB: 4.7 TB/s, a copy reaches 5.1) and the
-// sort and the rows' first places the rest.  131072 bf16 tokens of 256 bytes: 66 us, ten launches of 3 to 20 us that wait for
+// sort and the rows' first places the rest.  131072 bf16 tokens of 256 bytes: 56 us, eight launches of 3 to 20 us that wait for
 // each other; the sums would be 10 us at a copy's rate.  1000 tokens: 17 us, three launches.
 #include <algorithm>
 #include <math.h>
@@ -236,16 +236,6 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint2 *__restrict__ in,
         }
 }
 
-// first[v], the number of sorted keys below v, for v = 0 .. n_rows
-__global__ __launch_bounds__(256) void k_row_first(const uint2 *__restrict__ sorted, int32_t n, int64_t n_rows, int32_t *__restrict__ first)
-{
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v > n_rows) return;
-    int32_t lo = 0, hi = n;
-    while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (sorted[mid].x < (uint32_t)v) lo = mid + 1; else hi = mid; }
-    first[v] = lo;
-}
-
 // ------------------------------------------------------------------ sums
 // A row with more than 2^hs tokens is summed in stretches that start at multiples of 2^hs of the sorted list, so that many
 // groups of lanes share a popular row.  Such a row crosses a multiple of 2^hs, so a stretch holds at most two of them: the one
@@ -289,44 +279,61 @@ __device__ __forceinline__ void sum_rows(const T *__restrict__ grad, int64_t str
     }
 }
 
-// the row's parts k0 .. k1, of which the first is in slot 1 if the row starts inside it
+// parts k0 + g, k0 + g + step, .. k1 of a row, of which the first, k0, is in slot 1 if the row starts inside it
 template <int V>
 __device__ __forceinline__ void sum_parts(const float *__restrict__ parts, int32_t k0, int32_t k1, int64_t start, int64_t width, int32_t c,
-                                          int32_t d, float (&acc)[V])
+                                          int32_t d, float (&acc)[V], int g = 0, int step = 1)
 {
-    const float *src = parts + ((int64_t)k0 * 2 + ((int64_t)k0 * width < start)) * d + c;
-#pragma unroll
-    for (int q = 0; q < V; ++q) acc[q] += src[q];
-    src = parts + (int64_t)k0 * 2 * d + c;
+    const int64_t inside = (int64_t)k0 * width < start;
+    const float *src = parts + (int64_t)k0 * 2 * d + c;
     const int32_t m = k1 - k0;
 #pragma unroll 8
-    for (int32_t k = 1; k <= m; ++k)
+    for (int32_t k = g; k <= m; k += step)
 #pragma unroll
-        for (int q = 0; q < V; ++q) acc[q] += src[(int64_t)k * 2 * d + q];
+        for (int q = 0; q < V; ++q) acc[q] += src[(k ? (int64_t)k * 2 : inside) * d + q];
 }
 
+// Two things the sums need, in one launch.  The first `heavy_groups` workgroups sum the heavy rows' stretches, a group of L lanes
+// each; it finds what it has to know about its two rows in the keys around it: a row that holds a position of the stretch has
+// more than 2^hs tokens exactly if more than 2^hs of them lie no farther than 2^hs from the stretch.  The other workgroups write
+// first[v], the number of sorted keys below v, for v = 0 .. n_rows.
 template <typename T, int V, int L>
-__global__ __launch_bounds__(256) void k_heavy_parts(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t n,
-                                                     int64_t n_rows, int32_t d, const int32_t *__restrict__ first, int hs, float *__restrict__ parts)
+__global__ __launch_bounds__(256) void k_spread(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t n,
+                                                int64_t n_rows, int32_t d, int hs, int heavy_groups, float *__restrict__ parts, int32_t *__restrict__ first)
 {
-    const int gl = threadIdx.x % L;
-    const int32_t chunk = (int32_t)(group_id() * (256 / L) + threadIdx.x / L);
-    const int64_t lo = (int64_t)chunk << hs;
+    if (group_id() >= heavy_groups) {
+        const int64_t v = (group_id() - heavy_groups) * 256 + threadIdx.x;
+        if (v > n_rows) return;
+        int32_t lo = 0, hi = n;
+        while (lo < hi) { const int32_t mid = lo + ((hi - lo) >> 1); if (sorted[mid].x < (uint32_t)v) lo = mid + 1; else hi = mid; }
+        first[v] = lo;
+        return;
+    }
+    const int gl = threadIdx.x % L, width = 1 << hs;
+    const int64_t lo = (group_id() * (256 / L) + threadIdx.x / L) << hs;
     if (lo >= n) return;
-    const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + (1 << hs));
+    const int32_t a = (int32_t)lo, z = (int32_t)std::min<int64_t>(n, lo + width);
     const uint32_t kf = sorted[a].x, kl = sorted[z - 1].x;
+    uint32_t count = 0;                 // a byte each: tokens of kf near by, of kf in the stretch, of kl near by, of kl in the stretch
+    for (int i = gl; i < 3 * width; i += L) {
+        const int64_t t = lo - width + i;
+        if (t < 0 || t >= n) continue;
+        const uint32_t k = sorted[t].x, in = (t >= a && t < z) << 8 | 1;
+        count += (k == kf ? in : 0) + (k == kl ? in << 16 : 0);
+    }
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1) count += __shfl_xor(count, m, L);
 #pragma unroll 1
     for (int slot = 0; slot < 2; ++slot) {
-        const uint32_t kk = slot ? kl : kf;
-        if ((slot && kl == kf) || kk >= (uint64_t)n_rows) continue;
-        const int32_t s = first[kk], e = first[kk + 1];
-        if (e - s <= 1 << hs) continue;
+        const uint32_t kk = slot ? kl : kf, c2 = count >> (16 * slot);
+        if ((slot && kl == kf) || kk >= (uint64_t)n_rows || (int)(c2 & 255) <= width) continue;
+        const int32_t m = (c2 >> 8) & 255, s = slot ? z - m : a, e = s + m;
         for (int32_t c0 = 0; c0 < d; c0 += V * L) {
             const int32_t c = c0 + gl * V;
             float acc[V] = {};
-            sum_rows<T, V, L>(grad, stride, sorted, std::max(s, a), std::min(e, z), c, d, gl, acc);
+            sum_rows<T, V, L>(grad, stride, sorted, s, e, c, d, gl, acc);
             if (c < d) {
-                float *dst = parts + ((int64_t)chunk * 2 + slot) * d + c;
+                float *dst = parts + ((lo >> hs) * 2 + slot) * d + c;
 #pragma unroll
                 for (int q = 0; q < V; ++q) dst[q] = acc[q];
             }
@@ -357,7 +364,8 @@ __global__ __launch_bounds__(256) void k_super_parts(const uint2 *__restrict__ s
 }
 
 // The rows' sums.  The first `joins` workgroups join the parts of the heavy rows: a group of L lanes a stretch, for the heavy
-// row that starts in it (there is one at most: it goes on behind the stretch).  The others sum the light rows: a group takes R
+// row that starts in it (there is one at most: it goes on behind the stretch); a row of more than SUPER stretches, of which a
+// workgroup starts one at most, by all its groups, or (supers) from the sums of SUPER stretches.  The others sum the light rows: a group takes R
 // neighbouring rows, whose tokens are neighbours in the sorted list - one wait for the rows' first places, one for the tokens'
 // positions and one for every eight gradient rows, whichever row they belong to.  A table row has two or three tokens where the
 // batch is as long as the table, and a wait a step and row would be most of the time.
@@ -382,17 +390,45 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
     };
     const int64_t group = group_id();
     if (group < joins) {
+        __shared__ int32_t big[3];
+        __shared__ float sums[256 / L][V * L];
+        if (threadIdx.x == 0) big[2] = -1;
+        __syncthreads();
         const int64_t a = (group * (256 / L) + threadIdx.x / L) << hs;
-        if (a >= n) return;
-        const uint32_t v = sorted[std::min<int64_t>(n, a + (1 << hs)) - 1].x;
-        if (v >= (uint64_t)n_rows) return;
-        const int32_t s = first[v], e = first[v + 1];
-        if (e - s <= 1 << hs || s < a) return;
-        for (int32_t c = gl * V; c < d; c += V * L) {
+        const uint32_t v = a < n ? sorted[std::min<int64_t>(n, a + (1 << hs)) - 1].x : ~0u;
+        if (v < (uint64_t)n_rows) {
+            const int32_t s = first[v], e = first[v + 1];
+            if (e - s > 1 << hs && s >= a) {
+                const bool many = stretches(s, e, hs) > SUPER;
+                if (many && !supers) { if (gl == 0) { big[0] = s; big[1] = e; big[2] = (int32_t)v; } }
+                else
+                    for (int32_t c = gl * V; c < d; c += V * L) {
+                        float acc[V] = {};
+                        if (!many) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc);
+                        else sum_parts<V>(supers, s / (SUPER << hs), (e - 1) / (SUPER << hs), s, SUPER << hs, c, d, acc);
+                        put(acc, v, c, true);
+                    }
+            }
+        }
+        __syncthreads();
+        const int32_t s = big[0], e = big[1], row = big[2];
+        if (row < 0) return;
+        const int g = threadIdx.x / L;
+        for (int32_t c0 = 0; c0 < d; c0 += V * L) {
+            const int32_t c = c0 + gl * V;
             float acc[V] = {};
-            if (stretches(s, e, hs) <= SUPER) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc);
-            else sum_parts<V>(supers, s / (SUPER << hs), (e - 1) / (SUPER << hs), s, SUPER << hs, c, d, acc);
-            put(acc, v, c, true);
+            if (c < d) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc, g, 256 / L);
+#pragma unroll
+            for (int q = 0; q < V; ++q) sums[g][gl * V + q] = acc[q];
+            __syncthreads();
+            if (g == 0) {
+#pragma unroll 1
+                for (int k = 1; k < 256 / L; ++k)
+#pragma unroll
+                    for (int q = 0; q < V; ++q) acc[q] += sums[k][gl * V + q];
+                put(acc, row, c, true);
+            }
+            __syncthreads();
         }
         return;
     }
@@ -450,6 +486,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
 // what a gradient call keeps in its workspace
 struct GradPlan {
     int passes, bits, per, tiles, hs;
+    bool use_supers;
     int64_t sorted[2], counts, totals, first, parts, supers, bytes;
 };
 
@@ -476,7 +513,10 @@ GradPlan grad_plan(int64_t n, int64_t n_rows, int32_t d)
     // with 64), long ones write and read fewer parts (2 M tokens of fp32: 432, 405 and 402 us)
     p.hs = n <= RANK_MAX || n > 256 * 1024 ? 5 : 4;
     if (n > 1 << p.hs) p.parts = take(((n + (1 << p.hs) - 1) >> p.hs) * 2 * (int64_t)d * 4);
-    if (n > SUPER << p.hs) p.supers = take((n + (SUPER << p.hs) - 1) / (SUPER << p.hs) * 2 * (int64_t)d * 4);
+    // A row's parts joined by one workgroup, or first 32 and 32 of them in a launch of their own (131072 tokens of 59047 rows 56
+    // us, 61 with that launch, all of them of one row 77 and 61; 262144 of one row 167 and 87)
+    p.use_supers = n > 128 * 1024;
+    if (p.use_supers) p.supers = take((n + (SUPER << p.hs) - 1) / (SUPER << p.hs) * 2 * (int64_t)d * 4);
     p.bytes = std::max<int64_t>(at, 256);
     return p;
 }
@@ -490,9 +530,10 @@ template <typename T> struct SumArgs {
     int32_t d;
     float scale;
     int accumulate;
-    const int32_t *first;
+    int32_t *first;
+    bool has_first;                     // else it is to be found
     int hs;
-    float *parts, *supers;
+    float *parts, *supers;              // supers NULL: not used
     T *out;
     int64_t out_stride;
 };
@@ -501,19 +542,18 @@ template <typename T, int V, int L>
 int launch_sums(const SumArgs<T> &a, hipStream_t st)
 {
     constexpr int G = 256 / L;
-    int joins = 0;
-    if (a.n > 1 << a.hs) {
-        const int64_t chunks = ((int64_t)a.n + (1 << a.hs) - 1) >> a.hs;
-        joins = (int)((chunks + G - 1) / G);
-        hipLaunchKernelGGL((k_heavy_parts<T, V, L>), grid_of(joins), dim3(256), 0, st, a.grad, a.stride, a.sorted, a.n,
-                           a.n_rows, a.d, a.first, a.hs, a.parts);
-        if (a.n > SUPER << a.hs)
-            hipLaunchKernelGGL(k_super_parts, dim3((unsigned)((chunks + SUPER - 1) / SUPER)), dim3(256), 0, st, a.sorted, a.n, a.n_rows, a.d,
-                               a.first, a.hs, (const float *)a.parts, a.supers);
-    }
+    const int64_t chunks = a.n > 1 << a.hs ? ((int64_t)a.n + (1 << a.hs) - 1) >> a.hs : 0;
+    const int joins = (int)((chunks + G - 1) / G);
+    const int64_t spread = joins + (a.has_first ? 0 : (a.n_rows + 256) / 256);
+    if (spread)
+        hipLaunchKernelGGL((k_spread<T, V, L>), grid_of(spread), dim3(256), 0, st, a.grad, a.stride, a.sorted, a.n, a.n_rows, a.d, a.hs, joins,
+                           a.parts, a.first);
+    if (chunks && a.supers)
+        hipLaunchKernelGGL(k_super_parts, dim3((unsigned)((chunks + SUPER - 1) / SUPER)), dim3(256), 0, st, a.sorted, a.n, a.n_rows, a.d,
+                           (const int32_t *)a.first, a.hs, (const float *)a.parts, a.supers);
     constexpr int R = 4, per_group = G * R;           // rows a group (131072 tokens, 59047 rows: 66 us with 2 or 4, 74 with 8), rows a workgroup
     hipLaunchKernelGGL((k_row_sums<T, V, L, R>), grid_of(joins + (a.n_rows + per_group - 1) / per_group), dim3(256), 0, st, a.grad,
-                       a.stride, a.sorted, a.n, a.n_rows, a.d, a.scale, a.first, a.hs, joins, (const float *)a.parts, (const float *)a.supers, a.accumulate, a.out,
+                       a.stride, a.sorted, a.n, a.n_rows, a.d, a.scale, (const int32_t *)a.first, a.hs, joins, (const float *)a.parts, (const float *)a.supers, a.accumulate, a.out,
                        a.out_stride);
     MF_LAUNCH_CHECK();
     return MFSGD_OK;
@@ -561,10 +601,8 @@ int grad_impl(const T *grad, int64_t stride, const int32_t *ids, int64_t n, int6
                                     (const int32_t *)counts, (const int32_t *)totals, sorted[at]);
         }
     }
-    if (!has_first)
-        hipLaunchKernelGGL(k_row_first, dim3((unsigned)((n_rows + 256) / 256)), dim3(256), 0, st, (const uint2 *)sorted[at], m, n_rows, first);
-    const SumArgs<T> a = {grad, stride, sorted[at], m, n_rows, d, scale, accumulate, first, p.hs, (float *)(ws + p.parts), (float *)(ws + p.supers),
-                          out, out_stride};
+    const SumArgs<T> a = {grad, stride, sorted[at], m, n_rows, d, scale, accumulate, first, has_first, p.hs, (float *)(ws + p.parts),
+                          p.use_supers ? (float *)(ws + p.supers) : nullptr, out, out_stride};
     const int v = vec_elems(sizeof(T), d, stride, out_stride, grad, out);
     if constexpr (sizeof(T) == 2) {
         if (v == 8) return launch_sums_v<T, 8>(a, st);

@@ -119,7 +119,10 @@ def grad_want(grad, ids, rows, scale):
     (0, 5, 8, "even"), (1, 1, 1, "even"), (1, 7, 40, "even"), (63, 1000, 3, "even"), (64, 10, 100, "even"), (257, 1, 33, "even"),
     (300, 50, 128, "one"), (1000, 1682, 32, "popular"), (4095, 600, 129, "popular"), (4096, 1024, 64, "one"),
     (4097, 1023, 64, "popular"), (8192, 1024, 17, "one"), (20000, 17770, 128, "popular"), (30011, 59047, 200, "popular"),
-    (50000, 3, 256, "even"), (5000, 2000003, 4, "even"), (6000, 100, 520, "popular")])
+    (50000, 3, 256, "even"), (5000, 2000003, 4, "even"), (6000, 100, 520, "popular"),
+    # a row of many stretches: joined by one workgroup, then in two steps; rows that begin and end inside stretches
+    (131072, 9, 520, "one"), (20001, 70, 700, "popular"), (131073, 9, 40, "one"), (140003, 50, 36, "popular"), (300001, 1000, 33, "popular"),
+    (270000, 40000, 16, "popular")])
 def test_embedding_grad(dtype, n, rows, d, kind):
     g = gen(n + rows + d)
     grad = normal(g, n, d, dtype=dtype)
