@@ -301,7 +301,8 @@ int mfsgd_hip_als_step_f64(double *latent, const double *fixed, const int64_t *r
 int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows, int32_t d, const int32_t *ids, int64_t n,
                         float scale, int32_t dtype, void *out, void *stream);
 /* out[v] = scale * sum of grad[t] over the t with ids[t] == v, in the order of t; a row no id names is set to zero.
- * accumulate != 0: the sum is added to out[v] (rounded once), rows no id names stay as they are.  n < 2^31 - 1. */
+ * accumulate != 0: the sum is added to out[v] (rounded once), rows no id names stay as they are.  n <= 2^31 - 1024,
+ * d <= 2^30. */
 int64_t mfsgd_embedding_grad_workspace(int64_t n, int64_t n_rows, int32_t d);
 int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_t *ids, int64_t n, int64_t n_rows, int32_t d,
                              float scale, int32_t dtype, int32_t accumulate, void *out, int64_t out_stride,

@@ -242,6 +242,8 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint2 *__restrict__ in,
 // it starts with (slot 0) and another it ends with (slot 1).  The same again, SUPER stretches at a time, for rows of more than
 // SUPER stretches.
 constexpr int SUPER = 32;
+// a group's step behind the last token, or column, still fits 32 bits
+constexpr int64_t MAX_TOKENS = ((int64_t)1 << 31) - 1024, MAX_ROW = (int64_t)1 << 30;
 
 // Sum of grad[positions s .. e), columns c .. c + V of this lane; the group's L lanes read L positions at once and hand them round
 template <typename T, int V, int L>
@@ -631,7 +633,7 @@ int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows,
 
 int64_t mfsgd_embedding_grad_workspace(int64_t n, int64_t n_rows, int32_t d)
 {
-    if (n < 0 || n >= INT32_MAX || n_rows < 0 || n_rows >= INT32_MAX || d < 1) return -1;
+    if (n < 0 || n > MAX_TOKENS || n_rows < 0 || n_rows >= INT32_MAX || d < 1 || d > MAX_ROW) return -1;
     return grad_plan(n, n_rows, d).bytes;
 }
 
@@ -639,8 +641,8 @@ int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_
                              float scale, int32_t dtype, int32_t accumulate, void *out, int64_t out_stride, void *workspace,
                              int64_t workspace_bytes, void *stream)
 {
-    MF_ARG(n >= 0 && n < INT32_MAX && n_rows >= 0 && n_rows < INT32_MAX && d >= 1 && grad_stride >= d && out_stride >= d,
-           "embedding_grad: bad shape (n and the table below 2^31 - 1 rows)");
+    MF_ARG(n >= 0 && n <= MAX_TOKENS && n_rows >= 0 && n_rows < INT32_MAX && d >= 1 && d <= MAX_ROW && grad_stride >= d && out_stride >= d,
+           "embedding_grad: bad shape (n at most 2^31 - 1024, the table below 2^31 - 1 rows, rows of at most 2^30 elements)");
     MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "embedding_grad: unknown dtype %d", dtype);
     if (n_rows == 0 || (n == 0 && accumulate)) return MFSGD_OK;
     MF_ARG(out && (n == 0 || (grad && ids)), "embedding_grad: null pointer");

@@ -90,6 +90,9 @@ def test_c_refusals_embedding():
     assert need > 0
     assert lib.mfsgd_embedding_grad_workspace(-1, 100, 8) == -1
     assert lib.mfsgd_embedding_grad_workspace((1 << 31) - 1, 100, 8) == -1
+    assert lib.mfsgd_embedding_grad_workspace((1 << 31) - 1023, 100, 8) == -1 and lib.mfsgd_embedding_grad_workspace((1 << 31) - 1024, 100, 8) > 0
+    assert lib.mfsgd_embedding_grad_workspace(5000, 100, (1 << 30) + 1) == -1
+    assert "shape" in _refused(lib.mfsgd_hip_embedding_grad(p, 8, p, (1 << 31) - 1023, 100, 8, 1.0, 0, 0, p, 8, p, 1 << 50, None))
     assert "workspace" in _refused(lib.mfsgd_hip_embedding_grad(p, 8, p, 5000, 100, 8, 1.0, 0, 0, p, 8, p, need - 1, None))
     assert "workspace" in _refused(lib.mfsgd_hip_embedding_grad(p, 8, p, 5000, 100, 8, 1.0, 0, 0, p, 8, p + 4, need, None))
     assert "workspace" in _refused(lib.mfsgd_hip_embedding_grad(p, 8, p, 5000, 100, 8, 1.0, 0, 0, p, 8, None, need, None))
