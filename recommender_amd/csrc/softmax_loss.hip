@@ -159,7 +159,8 @@ template <int DP, int PL, int MODE, bool CONV> struct Shape {
     static constexpr int HOLD = CONV ? TB * CH / 256 : 0;            // pieces a thread holds on their way to LDS
     // registers: the stationary rows, the sums, the logits and what is in flight
     static constexpr int REGS = UT * PL * (DP - 16 * NB) / 4 + (MODE == LOSS ? 0 : UT * DP / 2) + UT * 16 + HOLD * (PL == 3 ? 8 : 4) + (CONV ? 20 : 0) + 48;
-    static constexpr int WAVES = REGS <= 120 ? 4 : REGS <= 156 ? 3 : REGS <= 256 ? 2 : 1;        // a SIMD
+    // waves a SIMD; at 256 (fp32 rows of 256, no gradients) two of them spill: 4096 x 17770 269 us, 220 with one
+    static constexpr int WAVES = REGS <= 120 ? 4 : REGS <= 156 ? 3 : REGS < 256 ? 2 : 1;
     static constexpr int GROUPS = WAVES < 160 * 1024 / LDS ? WAVES : 160 * 1024 / LDS;           // workgroups a CU
 };
 
