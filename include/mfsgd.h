@@ -297,7 +297,7 @@ int mfsgd_hip_als_step_f64(double *latent, const double *fixed, const int64_t *r
 #define MFSGD_F32 0
 #define MFSGD_BF16 1
 
-/* out[t] = scale * table[ids[t]], t < n; out is [n][d] without gaps.  Any d >= 1. */
+/* out[t] = scale * table[ids[t]], t < n; out is [n][d] without gaps.  1 <= d <= 2^30. */
 int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows, int32_t d, const int32_t *ids, int64_t n,
                         float scale, int32_t dtype, void *out, void *stream);
 /* out[v] = scale * sum of grad[t] over the t with ids[t] == v, in the order of t; a row no id names is set to zero.

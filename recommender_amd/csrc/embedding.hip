@@ -15,24 +15,31 @@
 
 namespace {
 
+// a group's step behind the last token, or column, still fits 32 bits
+constexpr int64_t MAX_TOKENS = ((int64_t)1 << 31) - 1024, MAX_ROW = (int64_t)1 << 30;
+
 // ------------------------------------------------------------------ lookup
-// A thread moves PIECES pieces of V elements (one access each), all of them asked for before the first one is used; the pieces
-// of the output are numbered through.  Bound by memory: 1 M bf16 rows of 200 bytes 42 us (5.1 TB/s, what a copy reaches; 96 us
+// A thread moves PIECES pieces of V elements (one access each), all of them asked for before
+// the first one is used; the pieces of the output are numbered through.  A row's last piece ends with the row: where V does not
+// divide the width it repeats some of the piece before, with the same values.  Bound by memory: 1 M bf16 rows of 200 bytes 42 us (5.1 TB/s, what a copy reaches; 96 us
 // with one piece a thread); 32 rows: the launch, 8.4 us from Python.
 constexpr int PIECES = 4;
-template <typename T, int V>
+template <typename T, int V, bool PAST>
 __global__ __launch_bounds__(256) void k_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d,
-                                                   const int32_t *__restrict__ ids, int64_t n, float scale, int past, T *out)
+                                                   const int32_t *__restrict__ ids, int64_t n, float scale, T *out)
 {
     constexpr int U = PIECES;
-    const int32_t per = d / V;
+    const int32_t per = (d + V - 1) / V;
     const int64_t p0 = group_id() * (256 * U), t0 = p0 / per;          // the same for all threads
     const int32_t skip = (int32_t)(p0 - t0 * per);
     int32_t id[U], c[U];
+    uint32_t to[U];                     // behind the first row's start: at most two rows and 1024 pieces
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t x = skip + u * 256 + threadIdx.x, row = x / (uint32_t)per;
-        c[u] = (int32_t)(x - row * per) * V;
+        const uint32_t x = skip + u * 256 + threadIdx.x;
+        const uint32_t row = x / (uint32_t)per;
+        c[u] = std::min((int32_t)(x - row * per) * V, d - V);
+        to[u] = row * (uint32_t)d + c[u];
         id[u] = ids[std::min<int64_t>(t0 + row, n - 1)];
     }
     float v[U][V];
@@ -44,8 +51,9 @@ __global__ __launch_bounds__(256) void k_embedding(const T *table, int64_t strid
 #pragma unroll
         for (int i = 0; i < V; ++i) v[u][i] = id[u] < 0 ? 0.f : id[u] < n_rows ? v[u][i] * scale : NAN;
         if (p < n * per) {
-            if (past) store_past<V>(out + p * V, v[u]);
-            else store_vec<V>(out + p * V, v[u]);
+            T *dst = out + t0 * d + to[u];
+            if constexpr (PAST) store_past<V>(dst, v[u]);
+            else store_vec<V>(dst, v[u]);
         }
     }
 }
@@ -55,19 +63,19 @@ int launch_embedding(const T *table, int64_t stride, int64_t n_rows, int32_t d, 
                      T *out, hipStream_t st)
 {
     if (n_rows == 0) { table = out; stride = 0; }       // nothing is taken from it, but the first piece is always asked for
-    const int v = vec_elems(sizeof(T), d, stride, d, table, out);
+    constexpr int WIDE = 16 / sizeof(T), HALF = 8 / sizeof(T);
+    // Pieces of 16 bytes where all of them are aligned, else of 8 (2 M bf16 rows of 254 bytes: 156 us by 8, 159 by 16 and 300 by
+    // elements; of 264 bytes: 155 by 8, 163 by 16)
+    const bool aligned = d % WIDE == 0 && stride % WIDE == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)out % 16 == 0;
+    const int v = aligned ? WIDE : d >= HALF ? HALF : 1;
     // A large output goes past the caches, which then hold the table: into memory not written lately 1 M rows of 200 bytes take 42
     // us against 68, 2 M of 512 bytes 224 against 321.  One that fits the L2s twice stays there for whoever reads it next
-    const int past = n * d * (int64_t)sizeof(T) > ((int64_t)64 << 20);
-    const dim3 grid = grid_of((n * (d / v) + 256 * PIECES - 1) / (256 * PIECES));
-#define MF_EMB(V_) hipLaunchKernelGGL((k_embedding<T, V_>), grid, dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, past, out)
-    if constexpr (sizeof(T) == 2) {
-        if (v == 8) { MF_EMB(8); MF_LAUNCH_CHECK(); return MFSGD_OK; }
-    }
-    if (v == 4) MF_EMB(4);
-    else if (v == 2) MF_EMB(2);
-    else MF_EMB(1);
-#undef MF_EMB
+    const bool past = n * d * (int64_t)sizeof(T) > ((int64_t)64 << 20);
+    const dim3 grid = grid_of((n * ((d + v - 1) / v) + 256 * PIECES - 1) / (256 * PIECES));
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, table, stride, n_rows, d, ids, n, scale, out); };
+    if (v == WIDE) go(past ? k_embedding<T, WIDE, true> : k_embedding<T, WIDE, false>);
+    else if (v == HALF) go(past ? k_embedding<T, HALF, true> : k_embedding<T, HALF, false>);
+    else go(past ? k_embedding<T, 1, true> : k_embedding<T, 1, false>);
     MF_LAUNCH_CHECK();
     return MFSGD_OK;
 }
@@ -242,15 +250,16 @@ __global__ __launch_bounds__(256) void k_sort_move(const uint2 *__restrict__ in,
 // it starts with (slot 0) and another it ends with (slot 1).  The same again, SUPER stretches at a time, for rows of more than
 // SUPER stretches.
 constexpr int SUPER = 32;
-// a group's step behind the last token, or column, still fits 32 bits
-constexpr int64_t MAX_TOKENS = ((int64_t)1 << 31) - 1024, MAX_ROW = (int64_t)1 << 30;
+
+// Lane gl of a group of L takes V columns, from here on; a row's last lane takes its last V, some of them another lane's as well
+__device__ __forceinline__ int32_t column(int32_t c, int32_t d, int V) { return std::min(c, d - V); }
 
 // Sum of grad[positions s .. e), columns c .. c + V of this lane; the group's L lanes read L positions at once and hand them round
 template <typename T, int V, int L>
 __device__ __forceinline__ void sum_rows(const T *__restrict__ grad, int64_t stride, const uint2 *__restrict__ sorted, int32_t s,
-                                         int32_t e, int32_t c, int32_t d, int gl, float (&acc)[V])
+                                         int32_t e, int32_t c, int gl, float (&acc)[V])
 {
-    const T *base = grad + (c < d ? c : 0);
+    const T *base = grad + c;
     for (int32_t a = s; a < e; a += L) {
         const int m = std::min<int32_t>(L, e - a);
         const int32_t mine = (int32_t)sorted[a + (gl < m ? gl : 0)].y;
@@ -290,9 +299,12 @@ __device__ __forceinline__ void sum_parts(const float *__restrict__ parts, int32
     const float *src = parts + (int64_t)k0 * 2 * d + c;
     const int32_t m = k1 - k0;
 #pragma unroll 8
-    for (int32_t k = g; k <= m; k += step)
+    for (int32_t k = g; k <= m; k += step) {
+        float v[V];
+        load_vec<V>(src + (k ? (int64_t)k * 2 : inside) * d, v);
 #pragma unroll
-        for (int q = 0; q < V; ++q) acc[q] += src[(k ? (int64_t)k * 2 : inside) * d + q];
+        for (int q = 0; q < V; ++q) acc[q] += v[q];
+    }
 }
 
 // Two things the sums need, in one launch.  The first `heavy_groups` workgroups sum the heavy rows' stretches, a group of L lanes
@@ -333,12 +345,8 @@ __global__ __launch_bounds__(256) void k_spread(const T *__restrict__ grad, int6
         for (int32_t c0 = 0; c0 < d; c0 += V * L) {
             const int32_t c = c0 + gl * V;
             float acc[V] = {};
-            sum_rows<T, V, L>(grad, stride, sorted, s, e, c, d, gl, acc);
-            if (c < d) {
-                float *dst = parts + ((lo >> hs) * 2 + slot) * d + c;
-#pragma unroll
-                for (int q = 0; q < V; ++q) dst[q] = acc[q];
-            }
+            sum_rows<T, V, L>(grad, stride, sorted, s, e, column(c, d, V), gl, acc);
+            if (c < d) store_vec<V>(parts + ((lo >> hs) * 2 + slot) * d + column(c, d, V), acc);
         }
     }
 }
@@ -380,12 +388,16 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
     const int gl = threadIdx.x % L;
     auto put = [&](float (&acc)[V], int64_t v, int32_t c, bool any) {
         if (c < d && (any || !accumulate)) {
-            T *dst = out + v * out_stride + c;
+            const int32_t c1 = column(c, d, V);
+            T *dst = out + v * out_stride + c1;
             float was[V] = {};
             if (accumulate) load_vec<V>(dst, was);
 #pragma unroll
             for (int q = 0; q < V; ++q) was[q] = fmaf(acc[q], scale, was[q]);
-            store_vec<V>(dst, was);
+            if (accumulate && c1 < c) {         // the columns of another lane: not a second time
+#pragma unroll
+                for (int q = 0; q < V; ++q) if (c1 + q >= c) store_f32(dst + q, was[q]);
+            } else store_vec<V>(dst, was);
         }
 #pragma unroll
         for (int q = 0; q < V; ++q) acc[q] = 0.f;
@@ -406,8 +418,8 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
                 else
                     for (int32_t c = gl * V; c < d; c += V * L) {
                         float acc[V] = {};
-                        if (!many) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc);
-                        else sum_parts<V>(supers, s / (SUPER << hs), (e - 1) / (SUPER << hs), s, SUPER << hs, c, d, acc);
+                        if (!many) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, column(c, d, V), d, acc);
+                        else sum_parts<V>(supers, s / (SUPER << hs), (e - 1) / (SUPER << hs), s, SUPER << hs, column(c, d, V), d, acc);
                         put(acc, v, c, true);
                     }
             }
@@ -419,7 +431,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
         for (int32_t c0 = 0; c0 < d; c0 += V * L) {
             const int32_t c = c0 + gl * V;
             float acc[V] = {};
-            if (c < d) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, c, d, acc, g, 256 / L);
+            if (c < d) sum_parts<V>(parts, s >> hs, (e - 1) >> hs, s, 1 << hs, column(c, d, V), d, acc, g, 256 / L);
 #pragma unroll
             for (int q = 0; q < V; ++q) sums[g][gl * V + q] = acc[q];
             __syncthreads();
@@ -445,7 +457,7 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
     for (int32_t c0 = 0; c0 < d; c0 += V * L) {
         const int32_t c = c0 + gl * V;
         float acc[V] = {};
-        const T *base = grad + (c < d ? c : 0);
+        const T *base = grad + column(c, d, V);
         for (int r = 0; r < rows; ++r) {
             if ((heavy >> r) & 1) continue;
             const int stop = std::min(rows, r + __builtin_ctz((heavy >> r) | 1u << R));     // rows r .. stop: none of them heavy
@@ -561,9 +573,12 @@ int launch_sums(const SumArgs<T> &a, hipStream_t st)
     return MFSGD_OK;
 }
 
-template <typename T, int V>
-int launch_sums_v(const SumArgs<T> &a, hipStream_t st)
+// Rows shorter than 16 bytes go by elements, others by pieces of 16 bytes
+template <typename T>
+int launch_sums_d(const SumArgs<T> &a, hipStream_t st)
 {
+    constexpr int V = 16 / sizeof(T);
+    if (a.d < V) return launch_sums<T, 1, 8>(a, st);
     const int lanes = (a.d + V - 1) / V;
     if (lanes <= 8) return launch_sums<T, V, 8>(a, st);
     if (lanes <= 16) return launch_sums<T, V, 16>(a, st);
@@ -605,13 +620,7 @@ int grad_impl(const T *grad, int64_t stride, const int32_t *ids, int64_t n, int6
     }
     const SumArgs<T> a = {grad, stride, sorted[at], m, n_rows, d, scale, accumulate, first, has_first, p.hs, (float *)(ws + p.parts),
                           p.use_supers ? (float *)(ws + p.supers) : nullptr, out, out_stride};
-    const int v = vec_elems(sizeof(T), d, stride, out_stride, grad, out);
-    if constexpr (sizeof(T) == 2) {
-        if (v == 8) return launch_sums_v<T, 8>(a, st);
-    }
-    if (v == 4) return launch_sums_v<T, 4>(a, st);
-    if (v == 2) return launch_sums_v<T, 2>(a, st);
-    return launch_sums_v<T, 1>(a, st);
+    return launch_sums_d(a, st);
 }
 
 }  // namespace
@@ -621,7 +630,7 @@ extern "C" {
 int mfsgd_hip_embedding(const void *table, int64_t table_stride, int64_t n_rows, int32_t d, const int32_t *ids, int64_t n,
                         float scale, int32_t dtype, void *out, void *stream)
 {
-    MF_ARG(n >= 0 && n_rows >= 0 && n_rows <= INT32_MAX && d >= 1 && table_stride >= d, "embedding: bad shape");
+    MF_ARG(n >= 0 && n_rows >= 0 && n_rows <= INT32_MAX && d >= 1 && d <= MAX_ROW && table_stride >= d, "embedding: bad shape");
     MF_ARG(dtype == MFSGD_F32 || dtype == MFSGD_BF16, "embedding: unknown dtype %d", dtype);
     if (n == 0) return MFSGD_OK;
     MF_ARG(n <= ((int64_t)1 << 40) / d, "embedding: more than 2^40 elements");

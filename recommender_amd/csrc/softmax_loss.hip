@@ -58,7 +58,7 @@ enum { LOSS = 0, LOSS_SUMS = 1, TABLE = 2 };   // pass 1 without / with the weig
 struct Rows {                           // rows as the caller has them
     const void *p;
     int64_t stride;
-    int32_t n, vec;                     // vec: elements a load may take
+    int32_t n;
 };
 
 struct StreamArgs {
@@ -77,24 +77,16 @@ struct StreamArgs {
     void *out;                          // pass 2: dW [n_items][d] of the rows' type, times out_f
     float *out_b;                       // and db, times weight
     float out_f, weight;
-    int32_t out_vec;
 };
 
 // 8 elements of a row from column c on, zero behind column d
 template <typename T> struct Piece;
 template <> struct Piece<float> { float v[8]; };
 template <> struct Piece<__bf16> { uint32_t v[4]; };
-__device__ __forceinline__ void load_piece(const float *row, int32_t c, int32_t d, int32_t vec, Piece<float> &o)
+__device__ __forceinline__ void load_piece(const float *row, int32_t c, int32_t d, Piece<float> &o)
 {
-    if (c + 8 <= d && vec >= 2) {
-        if (vec == 4) {
-            *(float4 *)(o.v) = *(const float4 *)(row + c);
-            *(float4 *)(o.v + 4) = *(const float4 *)(row + c + 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) *(float2 *)(o.v + i) = *(const float2 *)(row + c + i);
-        }
-    } else {
+    if (c + 8 <= d) load_vec<8>(row + c, o.v);
+    else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float t = row[c + i < d ? c + i : 0];
@@ -102,17 +94,12 @@ __device__ __forceinline__ void load_piece(const float *row, int32_t c, int32_t 
         }
     }
 }
-__device__ __forceinline__ void load_piece(const __bf16 *row, int32_t c, int32_t d, int32_t vec, Piece<__bf16> &o)
+__device__ __forceinline__ void load_piece(const __bf16 *row, int32_t c, int32_t d, Piece<__bf16> &o)
 {
-    if (c + 8 <= d && vec >= 2) {
-        if (vec == 8) *(uint4 *)o.v = *(const uint4 *)(row + c);
-        else if (vec == 4) {
-            *(uint2 *)o.v = *(const uint2 *)(row + c);
-            *(uint2 *)(o.v + 2) = *(const uint2 *)(row + c + 4);
-        } else {
+    if (c + 8 <= d) {
+        const words_of<8, __bf16> t = *(const words_of<8, __bf16> *)(row + c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o.v[i] = *(const uint32_t *)(row + c + 2 * i);
-        }
+        for (int i = 0; i < 4; ++i) o.v[i] = t[i];
     } else {
         const uint16_t *bits = (const uint16_t *)row;
 #pragma unroll
@@ -239,7 +226,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                 const int32_t row = t * TB + std::min(r, last);
                 const bool live = MODE == TABLE ? (uint32_t)a.targets[row] < (uint32_t)a.n_items : !a.bias || a.bias[row] != -INFINITY;
                 held |= (uint32_t)live << q;
-                load_piece((const T *)a.sm.p + row * a.sm.stride, c * 8, a.d, a.sm.vec, hold[q]);
+                load_piece((const T *)a.sm.p + row * a.sm.stride, c * 8, a.d, hold[q]);
             }
         } else {
             const __bf16 *base = a.sm_planes + (int64_t)t * TB * a.planes_stride;
@@ -356,7 +343,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
         for (int s = 0; s < KS; ++s) {
             Piece<T> raw;
             bf16x8 v[PL];
-            load_piece((const T *)a.st.p + row * a.st.stride, 16 * s + 8 * kh, a.d, a.st.vec, raw);
+            load_piece((const T *)a.st.p + row * a.st.stride, 16 * s + 8 * kh, a.d, raw);
             split_piece(raw, live, v);
 #pragma unroll
             for (int p = 0; p < PL; ++p) {
@@ -611,7 +598,7 @@ __global__ __launch_bounds__(256, (Shape<DP, sizeof(T) == 4 ? 3 : 1, MODE, CONV>
                         float v[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = o[u][dt][4 * j + i] * a.out_f;
-                        if (a.out_vec >= 4) store_vec<4>(dst, v);
+                        if (c + 4 <= a.d) store_vec<4>(dst, v);
                         else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) if (c + i < a.d) store_f32(dst + i, v[i]);
@@ -644,7 +631,7 @@ __global__ __launch_bounds__(256) void k_planes(const PlaneJob x, const PlaneJob
     const bool live = is_x ? (uint32_t)job.targets[r] < (uint32_t)n_items : !job.bias || job.bias[r] != -INFINITY;
     Piece<T> raw;
     bf16x8 v[PL];
-    load_piece((const T *)job.src.p + r * job.src.stride, c, d, job.src.vec, raw);
+    load_piece((const T *)job.src.p + r * job.src.stride, c, d, raw);
     split_piece(raw, live, v);
 #pragma unroll
     for (int q = 0; q < PL; ++q) *(bf16x8 *)(job.dst + (int64_t)q * n * dp + r * dp + c) = v[q];
@@ -766,9 +753,14 @@ __global__ __launch_bounds__(256) void k_join_items(const float *__restrict__ pa
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int k = 0; k < splits; ++k) s += *(const f32x4 *)(part_o + ((int64_t)k * n_items + v) * dp + c);
+    float o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c + i < d) store_f32(dw + v * d + c + i, s[i] * f);
+    for (int i = 0; i < 4; ++i) o[i] = s[i] * f;
+    if (c + 4 <= d) store_vec<4>(dw + v * d + c, o);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < d) store_f32(dw + v * d + c + i, o[i]);
     if (db && c == 0) {
         float t = 0.f;
         for (int k = 0; k < splits; ++k) t += part_s[(int64_t)k * n_items + v];
@@ -889,10 +881,9 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
 {
     constexpr int PL = sizeof(T) == 4 ? 3 : 1;
     const LossPlan p = loss_plan(n, n_items, d, PL == 3 ? MFSGD_F32 : MFSGD_BF16, grads);
-    const Rows xr = {x, xs, (int32_t)n, vec_elems(sizeof(T), 16, xs, xs, x, x)};
-    const Rows wr = {w, ws_, (int32_t)n_items, vec_elems(sizeof(T), 16, ws_, ws_, w, w)};
+    const Rows xr = {x, xs, (int32_t)n}, wr = {w, ws_, (int32_t)n_items};
     // a bf16 table whose rows are dp wide and start at multiples of 16 bytes is the operand as it is
-    const bool as_is = PL == 1 && d == p.dp && wr.vec == 8 && ws_ < (1 << 20);
+    const bool as_is = PL == 1 && d == p.dp && ws_ % 8 == 0 && (uintptr_t)w % 16 == 0 && ws_ < (1 << 20);
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
     if (!p.conv) {
         auto groups = [&](int64_t rows) { return (rows * (p.dp / 8) + 255) / 256; };
@@ -944,7 +935,6 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     a.part_o = p.splits2 > 1 ? (float *)(ws + p.o2) : nullptr;
     a.row_init = j.row_init; a.row_q = j.row_q; a.row_g = j.row_g;
     a.out = dw; a.out_b = db; a.out_f = scale * weight; a.weight = weight;
-    a.out_vec = vec_elems(sizeof(T), d, d, d, dw, dw);
     if (const int rc = launch_stream_d<T, TABLE>(p.dp, p.conv, a, st)) return rc;
     if (p.splits2 > 1) {
         hipLaunchKernelGGL((k_join_items<T>), grid_of((n_items * ((d + 3) / 4) + 255) / 256), dim3(256), 0, st, a.part_o, a.part_s, p.splits2, n_items,

@@ -45,7 +45,9 @@ def close(got, want, tol):
 # ------------------------------------------------------------------ lookup
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n, rows, d, pad", [(1, 1, 1, 0), (7, 5, 3, 0), (33, 100, 40, 24), (1000, 37, 100, 0), (257, 1000, 128, 0),
-                                             (64, 20, 129, 1), (5000, 3000, 256, 0), (3, 10, 1000, 6)])
+                                             (64, 20, 129, 1), (5000, 3000, 256, 0), (3, 10, 1000, 6),
+                                             (500, 60, 4, 0), (500, 60, 5, 2), (500, 60, 7, 1), (501, 60, 8, 3), (501, 60, 9, 0),
+                                             (333, 60, 127, 0), (333, 60, 130, 1), (12, 60, 1031, 0), (300000, 60, 131, 0)])
 def test_embedding(dtype, n, rows, d, pad):
     g = gen(n + d)
     table = normal(g, rows, d + pad, dtype=dtype)[:, :d]
@@ -122,7 +124,10 @@ def grad_want(grad, ids, rows, scale):
     (50000, 3, 256, "even"), (5000, 2000003, 4, "even"), (6000, 100, 520, "popular"),
     # a row of many stretches: joined by one workgroup, then in two steps; rows that begin and end inside stretches
     (131072, 9, 520, "one"), (20001, 70, 700, "popular"), (131073, 9, 40, "one"), (140003, 50, 36, "popular"), (300001, 1000, 33, "popular"),
-    (270000, 40000, 16, "popular")])
+    (270000, 40000, 16, "popular"),
+    # widths that no piece of 16 bytes divides; a row's last piece alone in its round
+    (900, 300, 515, "popular"), (900, 300, 258, "popular"), (6000, 3, 515, "one"), (6000, 4, 259, "even"), (5000, 3, 9, "popular"),
+    (3000, 700, 127, "popular"), (9000, 5, 5, "popular"), (700, 90, 7, "even")])
 def test_embedding_grad(dtype, n, rows, d, kind):
     g = gen(n + rows + d)
     grad = normal(g, n, d, dtype=dtype)
