@@ -674,20 +674,23 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
         for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
         z = (wave_sum(dot) * a.scale + bias) * LOG2E;
     }
+    // The largest part's sum, log2.  Not the largest of the parts' references: a sum may stand 2^60 above its own
     float m = -INFINITY;
     bool bad = false;
     for (int s = lane; s < a.splits; s += 64) {
-        m = fmaxf(m, a.part_m[(int64_t)s * a.n + r]);
-        bad |= !(a.part_s[(int64_t)s * a.n + r] >= 0.f);       // not a number
+        const float v = a.part_s[(int64_t)s * a.n + r];
+        m = fmaxf(m, a.part_m[(int64_t)s * a.n + r] + __builtin_amdgcn_logf(v));
+        bad |= !(v >= 0.f);                                    // not a number
     }
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
     const float top = fmaxf(m, z);
     const bool none = z == -INFINITY && !__ballot(bad);        // the target, or every item, is out of the catalogue: no gradient
     const bool empty = none && m == -INFINITY;
-    // Everything relative to the target's logit unless it lies so far below that the others' share would overflow: the loss is
-    // then log1p(others), with no difference of nearly equal numbers in it
-    const bool near = z > m - 64.f;
+    // Everything relative to the largest of the target's exponential and the parts' sums: a part's sum and its weighted sums are
+    // then multiplied by no more than what makes that sum at most 1.  Where it is the target's the loss is log1p(others), with no
+    // difference of nearly equal numbers in it; elsewhere it is a sum of two numbers of one sign
+    const bool near = z > m;
     const float ref = near ? z : (top == -INFINITY ? 0.f : top);
     float sum = 0.f;
     for (int s = lane; s < a.splits; s += 64) sum += a.part_s[(int64_t)s * a.n + r] * __builtin_amdgcn_exp2f(a.part_m[(int64_t)s * a.n + r] - ref);

@@ -412,6 +412,52 @@ def test_softmax_loss_large_logits():
             close(got[k], out[k], tol[k])
 
 
+def far_below_case(n, items, d, dtype, wide, high):
+    """Logits of nearly nothing but the bias: 0, 40 on the items `high` (e^40 is below 2^58), -44 on the targets, last items."""
+    g = gen(items + d)
+    x, w = normal(g, n, d, dtype=dtype, std=1e-4), normal(g, items, d, dtype=dtype, std=wide)
+    b = torch.zeros(items, device="cuda")
+    b[high] = 40.0
+    t = (items - 1 - torch.arange(n, device="cuda") % 3).int()
+    b[items - 3:] = -44.0
+    return x, w, t, b, torch.rand(n, device="cuda", generator=g) + 0.5
+
+
+def far_below_holds(x, w, t, b, each):
+    n, (items, d) = x.shape[0], w.shape
+    out, mass = loss_want(x, w, t, b, 1.0, each)
+    assert float(out[0].min()) > 80
+    tol = loss_tolerances(out, mass, n, items, d, x.dtype)
+    loss, lse = ra.softmax_loss(x, w, t, bias=b)
+    close(loss, out[0], tol[0])
+    close(lse, out[1], tol[1])
+    got = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+    for k in range(5):
+        close(got[k], out[k], tol[k])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, d, wide", [(5, 8, 400.0), (5, 8, 1.0), (3, 128, 30.0), (140, 40, 400.0)])
+def test_softmax_loss_target_far_below(dtype, n, d, wide):
+    """The first items set a low reference, the sum stands 2^58 above it and the target 2^63 below: fp32 has to hold what the
+    join makes of them, times the items' elements."""
+    far_below_holds(*far_below_case(n, 64, d, dtype, wide, [50]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", [(1, 17770, 128), (40, 9000, 40), (700, 9000, 64)])
+def test_softmax_loss_target_far_below_many_parts(dtype, n, items, d):
+    """... and the sums of many parts of the items, of which each starts at a multiple of 32 or 64 items and is as far above its
+    first ones: whatever the number of parts is, one of these inputs has the high items behind the start of all of them."""
+    for tile in (32, 64):
+        tiles = (items + tile - 1) // tile
+        for parts in (8, 16, 24, 32, 48, 64, 96, 128, 192, 256):
+            starts = {tiles * k // parts for k in range(parts)}
+            high = [k * tile + tile // 2 + 3 if tile == 64 else (k + 1) * tile + 3 for k in starts]
+            high = [i for i in high if i < items - 3 and (tile == 64 or i // tile not in starts)]
+            far_below_holds(*far_below_case(n, items, d, dtype, 1.0, high))
+
+
 def test_softmax_loss_strides():
     g = gen(11)
     n, items, d = 37, 90, 64
