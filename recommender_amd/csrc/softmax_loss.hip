@@ -673,6 +673,7 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
         float dot = 0.f;
         for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
         z = (wave_sum(dot) * a.scale + bias) * LOG2E;
+        if (z == INFINITY) z = NAN;                            // inf - inf: pass 1, which leaves the target out, does not show it
     }
     // The largest part's sum, log2.  Not the largest of the parts' references: a sum may stand 2^60 above its own
     float m = -INFINITY;

@@ -458,6 +458,27 @@ def test_softmax_loss_target_far_below_many_parts(dtype, n, items, d):
             far_below_holds(*far_below_case(n, items, d, dtype, 1.0, high))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", [(1, 3, 8), (40, 100, 32), (3, 5000, 128), (700, 300, 64)])
+@pytest.mark.parametrize("how", ["row", "bias", "product"])
+def test_softmax_loss_infinite_target_shows(dtype, n, items, d, how):
+    """The target's logit is +inf: lse - z is not a number, and the row is not a perfectly learnt one."""
+    for at in {2, min(items - 1, 50), items - 1}:
+        x, w, t, b = loss_case(gen(at), n, items, d, dtype, True)
+        t[:] = (at + 1) % items
+        t[0], x[0, 2] = at, 1.5
+        if how == "row":
+            w[at, 2] = math.inf
+        elif how == "bias":
+            b[at] = math.inf
+        else:
+            x[0, 2], w[at, 2] = 1e30, 1e30
+        loss, lse = ra.softmax_loss(x, w, t, bias=b)
+        assert math.isnan(float(loss[0])) and not math.isfinite(float(lse[0])), at
+        loss, lse, dx, _, _ = ra.softmax_loss_grads(x, w, t, bias=b)
+        assert math.isnan(float(loss[0])) and not math.isfinite(float(lse[0])) and bool(torch.isnan(dx[0]).all()), at
+
+
 def test_softmax_loss_strides():
     g = gen(11)
     n, items, d = 37, 90, 64
