@@ -313,7 +313,8 @@ int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_
  *   lse[r] = log sum_v exp z_rv,   loss[r] = lse[r] - z_{r, targets[r]}.
  * A bias of -inf takes an item out of the catalogue, whatever its row holds; a row whose target is out has the loss +inf and
  * no gradient, with every item out also the lse -inf.  A padding row's x is not looked at: loss and lse are 0.
- * A logit of a row that is +inf (2.3e38 and more count as that) or not a number makes its loss, lse and gradients not a number.
+ * A logit of a row that is +inf (2.3e38 and more count as that) or not a number makes its loss, lse and gradients not a number;
+ * so may any logit of an infinite float32 element.  A target whose logit is -inf otherwise has the loss +inf and probability 0.
  * 1e-20 <= scale <= 1e20, and bias / scale and bias * log2(e) have to be finite in float32 (or the bias -inf). */
 int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads);
 int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets,

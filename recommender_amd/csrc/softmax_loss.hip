@@ -669,7 +669,8 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
     }
     const float bias = a.bias ? a.bias[t] : 0.f;
     float z = -INFINITY;                                       // the target's logit, log2
-    if (bias != -INFINITY) {
+    const bool out = bias * LOG2E == -INFINITY;                // the target is out of the catalogue
+    if (!out) {
         float dot = 0.f;
         for (int c = lane; c < a.d; c += 64) dot = fmaf(load_f32(x + r * a.x_stride + c), load_f32(w + (int64_t)t * a.w_stride + c), dot);
         z = (wave_sum(dot) * a.scale + bias) * LOG2E;
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
     const float top = fmaxf(m, z);
-    const bool none = z == -INFINITY && !__ballot(bad);        // the target, or every item, is out of the catalogue: no gradient
+    const bool none = out && !__ballot(bad);                   // no gradient
     const bool empty = none && m == -INFINITY;
     // Everything relative to the largest of the target's exponential and the parts' sums: a part's sum and its weighted sums are
     // then multiplied by no more than what makes that sum at most 1.  Where it is the target's the loss is log1p(others), with no

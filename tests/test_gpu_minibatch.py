@@ -479,6 +479,37 @@ def test_softmax_loss_infinite_target_shows(dtype, n, items, d, how):
         assert math.isnan(float(loss[0])) and not math.isfinite(float(lse[0])) and bool(torch.isnan(dx[0]).all()), at
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", [(1, 3, 8), (40, 100, 32), (3, 5000, 128), (700, 300, 64)])
+def test_softmax_loss_target_without_probability(dtype, n, items, d):
+    """A target of the catalogue whose logit is -inf: an infinite loss, and the gradient of probability 0, not none.  An fp32
+    element is the sum of three bf16 ones, and -inf less its first part is not a number: there it may show as that instead."""
+    for at in {2, min(items - 1, 50), items - 1}:
+        x, w, t, b = loss_case(gen(at), n, items, d, dtype, True)
+        t[:], x[:, 2], w[at, 2] = at, 1.5, -math.inf
+        loss, lse = ra.softmax_loss(x, w, t, bias=b)
+        got, _, dx, dw, db = ra.softmax_loss_grads(x, w, t, bias=b, weights=0.5)
+        assert not bool(torch.isfinite(torch.cat([loss, got, dx[:, 2]])).any()), at
+        if dtype == F32:
+            assert not bool(torch.isfinite(dw[at]).any()) or float(dw[at].abs().sum()) > 0
+            continue
+        assert bool((loss == math.inf).all()) and bool((got == math.inf).all()) and bool(torch.isfinite(lse).all()), at
+        want = -0.5 * x.double().sum(0)
+        close(dw[at], want, half(dtype) * want.abs() + (n + 8) * U * 0.5 * x.double().abs().sum(0))
+        assert abs(float(db[at]) + 0.5 * n) <= n * n * U
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", [(1, 3, 8), (40, 100, 32), (3, 5000, 128), (700, 300, 64)])
+def test_softmax_loss_infinite_item_shows(dtype, n, items, d):
+    """An item's logit of +inf that is no row's target."""
+    for at in {2, min(items - 1, 50), items - 1}:
+        x, w, t, b = loss_case(gen(at), n, items, d, dtype, True)
+        t[:], x[:, 2], w[at, 2] = (at + 1) % items, 1.5, math.inf
+        for loss, lse, *_ in (ra.softmax_loss(x, w, t, bias=b), ra.softmax_loss_grads(x, w, t, bias=b)):
+            assert bool(torch.isnan(loss).all()) and bool(torch.isnan(lse).all()), at
+
+
 def test_softmax_loss_strides():
     g = gen(11)
     n, items, d = 37, 90, 64
