@@ -31,14 +31,17 @@ def bytes_per_update(k, implicit):
 
 def kernel_source_hash():
     """Identifies the build a PMC record in profiles/traffic.json belongs to: sha256 over the sources of the epoch kernel
-    (csrc/epoch.hip, csrc/common.h - the GPU box has no .git).  profiles/collect_traffic.py stores the same hash with
-    every record it writes."""
+    (csrc/epoch.hip, csrc/common.h - the GPU box has no .git) and the compiler flags that the Makefile gives them.
+    profiles/collect_traffic.py stores the same hash with every record it writes."""
     import hashlib
+    import re
     h = hashlib.sha256()
+    csrc = os.path.join(ROOT, "recommender_amd", "csrc")
     for name in ("epoch.hip", "common.h"):
-        path = os.path.join(ROOT, "recommender_amd", "csrc", name)
         h.update(name.encode())
-        h.update(open(path, "rb").read())
+        h.update(open(os.path.join(csrc, name), "rb").read())
+    flags = re.findall(r"^(?:override )?(?:ARCH|CXXFLAGS|NO_PACKED_FP32|COMPILE) *[:?]?=.*", open(os.path.join(csrc, "Makefile")).read(), re.M)
+    h.update("\n".join(flags).encode())
     return h.hexdigest()[:16]
 
 

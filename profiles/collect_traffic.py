@@ -6,7 +6,7 @@
 key = the one bench.py looks up: workload/k<k>/<implicit>/<Gr>x<Gc>/hot<hot_buffers>.  Per launch of k_epoch_free:
 bytes = (2 * FETCH_SIZE + WRITE_SIZE) * 1024 - on gfx950 FETCH_SIZE reports half of a coalesced read stream
 (MI355X_MICROARCH.md, HBM section; calibrated in round 1 against the known P-row volume).  The record carries the hash
-of the kernel sources (bench.kernel_source_hash), and bench.py quotes it only for a build with the same hash.
+of the kernel's sources and compiler flags (bench.kernel_source_hash), and bench.py quotes it only for a build with the same hash.
 """
 import csv
 import glob
@@ -37,7 +37,7 @@ write, nw = counter_mean(os.path.join(d, "write"), "WRITE_SIZE")
 path = os.path.join(ROOT, "profiles", "traffic.json")
 db = json.load(open(path))
 db[key] = {"fetch_kb": round(fetch, 1), "write_kb": round(write, 1), "traffic_bytes": int((2 * fetch + write) * 1024),
-           "launches": [nf, nw], "source_hash": kernel_source_hash(), "round": 3,
+           "launches": [nf, nw], "source_hash": kernel_source_hash(),
            "note": sys.argv[3] if len(sys.argv) > 3 else ""}
 json.dump(db, open(path, "w"), indent=2)
 print(key, db[key])
