@@ -640,10 +640,12 @@ class ExplicitMF(Recommender):
         """One minibatch step of the ranking objective that `top_n` answers for: lowers the mean over the batch of
         -log softmax(scale * user_vecs[users] @ item_vecs.T + b_i)[items], in place on the given ROCm tensors (float32 or
         bfloat16 factors, float32 b_i; users and items int32, a user or an item < 0 is padding, one behind its table gives a
-        loss that is not a number and no gradient).  With `max_norm` the gradients of all factors are clipped to it first.
+        loss that is not a number and no gradient).  NumPy arrays are refused: there would be nothing to update in place.  With
+        `max_norm` the gradients of all factors are clipped to it first.
         Returns (loss [n], norm of the gradients); asynchronous, no host copies."""
-        from .minibatch import clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
+        from .minibatch import check_step, clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
         torch = _abi.torch_mod()
+        check_step(users, items, user_vecs, item_vecs, b_i)
         n = int(users.shape[0])
         # a row whose user is no row of user_vecs must not reach the items' gradients
         items = torch.where(users < 0, users, torch.where(users < user_vecs.shape[0], items, 2 ** 31 - 1))

@@ -267,3 +267,22 @@ def clip_grads(tensors, max_norm, out=None):
         _abi.check(_abi.lib().mfsgd_hip_clip_grads(grads.addresses.buffer_info()[0], to.addresses.buffer_info()[0], sizes, dtypes, n,
                                                    max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), on.stream))
     return norm
+
+
+def check_step(users, items, user_vecs, item_vecs, b_i):
+    """What ExplicitMF.ranking_step takes, checked before anything runs: a step is done whole or not at all."""
+    for t, name in ((users, "users"), (items, "items")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+            raise TypeError(f"ranking_step: {name} must be an int32 ROCm tensor")
+        if t.dim() != 1 or t.shape != users.shape:
+            raise ValueError("ranking_step: users and items must have one dimension and the same length")
+    for t, name in ((user_vecs, "user_vecs"), (item_vecs, "item_vecs")):
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
+            raise TypeError(f"ranking_step: {name} must be a float32 or bfloat16 ROCm tensor, which is updated in place")
+    if user_vecs.dim() != 2 or item_vecs.dim() != 2 or user_vecs.shape[1] != item_vecs.shape[1] or user_vecs.dtype != item_vecs.dtype:
+        raise ValueError("ranking_step: user_vecs and item_vecs must have rows of one length and type")
+    if b_i is not None:
+        if not isinstance(b_i, torch.Tensor) or b_i.dtype != torch.float32:
+            raise TypeError("ranking_step: b_i must be a float32 ROCm tensor, which is updated in place")
+        if b_i.shape != item_vecs.shape[:1]:
+            raise ValueError("ranking_step: b_i must have an element for every item")

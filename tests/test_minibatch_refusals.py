@@ -4,6 +4,7 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -63,6 +64,21 @@ def test_out_must_not_overlap():
     both = torch.zeros(8, 8)
     with pytest.raises(ValueError, match="overlap"):
         ra.embedding_grad(both[:4], _i(0, 1, 2, 3), 4, out=both[2:6])
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(users=np.zeros(4, np.int32)), TypeError), (dict(items=[0, 1, 2, 3]), TypeError),
+    (dict(users=torch.zeros(4, dtype=torch.int64)), TypeError), (dict(items=torch.zeros(4)), TypeError),
+    (dict(user_vecs=np.zeros((9, 8), np.float32)), TypeError), (dict(item_vecs=np.zeros((5, 8))), TypeError),
+    (dict(user_vecs=_x(9).double()), TypeError), (dict(b_i=np.zeros(5)), TypeError), (dict(b_i=torch.zeros(5).bfloat16()), TypeError),
+    (dict(items=_i(0)), ValueError),                                            # one item for all users: not broadcast
+    (dict(users=_i(0)), ValueError), (dict(users=_i(0, 1, 2, 3).view(2, 2), items=_i(0, 1, 2, 3).view(2, 2)), ValueError),
+    (dict(user_vecs=_x(9, 7)), ValueError), (dict(user_vecs=_x(9, 8, torch.bfloat16)), ValueError), (dict(item_vecs=torch.zeros(8)), ValueError),
+    (dict(b_i=torch.zeros(9)), ValueError), (dict(b_i=torch.zeros(1)), ValueError)])
+def test_ranking_step_refusals(change, error):
+    given = dict(users=_i(0, 1, 2, 3), items=_i(0, 1, 2, 3), user_vecs=_x(9), item_vecs=_x(5), b_i=torch.zeros(5))
+    with pytest.raises(error, match="ranking_step"):
+        ra.ExplicitMF.ranking_step(**{**given, **change})
 
 
 def test_no_gpu_no_answer():
