@@ -655,8 +655,9 @@ class ExplicitMF(Recommender):
         pairs = [(user_vecs, dp), (item_vecs, dq)] + ([(b_i, db)] if b_i is not None else [])
         grads = [g for _, g in pairs]
         norm = grad_norm(grads) if max_norm is None else clip_grads(grads, max_norm)
-        for t, g in pairs:
-            t.sub_(g, alpha=lr)
+        with torch.no_grad():                   # tables that require gradients are updated like any
+            for t, g in pairs:
+                t.sub_(g, alpha=lr)
         return loss, norm
 
     def recommend(self, users, n=10):

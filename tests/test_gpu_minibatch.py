@@ -669,6 +669,19 @@ def test_ranking_step_users_out_of_range():
     assert torch.equal(loss, want) and all(torch.equal(x, y) for x, y in zip(one, two))
 
 
+def test_ranking_step_tables_that_require_gradients():
+    """All of them or one: the same step, and none of it recorded."""
+    for which in ((0, 1, 2), (1,), (2,)):
+        u, i, *tables = batch(37)
+        plain = [t.clone() for t in tables]
+        for k in which:
+            tables[k].requires_grad_()
+        loss, norm = ra.ExplicitMF.ranking_step(u, i, *tables, max_norm=0.05)
+        want, length = ra.ExplicitMF.ranking_step(u, i, *plain, max_norm=0.05)
+        assert torch.equal(loss, want) and torch.equal(norm, length) and not loss.requires_grad
+        assert all(torch.equal(a, b) and a.grad_fn is None for a, b in zip(tables, plain))
+
+
 def test_captured_step_replays():
     """The whole step in a graph, replayed on new inputs with eager work of the same kind in between."""
     u, i, P, Q, b = batch(31, n=5000)
