@@ -640,10 +640,11 @@ class ExplicitMF(Recommender):
         """One minibatch step of the ranking objective that `top_n` answers for: lowers the mean over the batch of
         -log softmax(scale * user_vecs[users] @ item_vecs.T + b_i)[items], in place on the given ROCm tensors (float32 or
         bfloat16 factors, float32 b_i; users and items int32, a user or an item < 0 is padding, one behind its table gives a
-        loss that is not a number and no gradient).  NumPy arrays are refused: there would be nothing to update in place.  With
-        `max_norm` the gradients of all factors are clipped to it first.
+        loss that is not a number and no gradient).  NumPy arrays are refused: there would be nothing to update in place; so
+        are tensors that share memory, but for one table as both: its gradients are added up.  With `max_norm` the gradients of
+        all factors are clipped to it first.
         Returns (loss [n], norm of the gradients); asynchronous, no host copies."""
-        from .minibatch import check_step, clip_grads, embedding, embedding_grad, grad_norm, softmax_loss_grads
+        from .minibatch import check_step, clip_grads, embedding, embedding_grad, grad_norm, same_table, softmax_loss_grads
         torch = _abi.torch_mod()
         check_step(users, items, user_vecs, item_vecs, b_i)
         n = int(users.shape[0])
@@ -651,8 +652,11 @@ class ExplicitMF(Recommender):
         items = torch.where(users < 0, users, torch.where(users < user_vecs.shape[0], items, 2 ** 31 - 1))
         x = embedding(user_vecs, users)
         loss, _, dx, dq, db = softmax_loss_grads(x, item_vecs, items, bias=b_i, scale=scale, weights=1.0 / max(n, 1))
-        dp = embedding_grad(dx, users, user_vecs.shape[0])
-        pairs = [(user_vecs, dp), (item_vecs, dq)] + ([(b_i, db)] if b_i is not None else [])
+        if same_table(user_vecs, item_vecs):
+            pairs = [(item_vecs, embedding_grad(dx, users, user_vecs.shape[0], out=dq, accumulate=True))]
+        else:
+            pairs = [(user_vecs, embedding_grad(dx, users, user_vecs.shape[0])), (item_vecs, dq)]
+        pairs += [(b_i, db)] if b_i is not None else []
         grads = [g for _, g in pairs]
         norm = grad_norm(grads) if max_norm is None else clip_grads(grads, max_norm)
         with torch.no_grad():                   # tables that require gradients are updated like any

@@ -91,6 +91,20 @@ def _overlap(a, b):
     return x is not None and y is not None and x[0] < y[1] and y[0] < x[1]
 
 
+def _share(a, b):
+    """Whether two tensors have elements in common.  Columns of one wider table have not, though their spans overlap; other
+    tensors with overlapping spans are taken to."""
+    if not _overlap(a, b):
+        return False
+    wide = a.stride(0)
+    if a.dtype != b.dtype or b.stride(0) != wide or any(t.dim() == 2 and t.shape[1] > 1 and t.stride(1) != 1 for t in (a, b)):
+        return True
+    apart, rest = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    widths = [t.shape[1] if t.dim() == 2 else 1 for t in (a, b)]
+    apart %= max(wide, 1)                               # b's columns begin here in a's rows, and a's next row behind them
+    return bool(rest) or apart < widths[0] or apart + widths[1] > wide
+
+
 def embedding(table, ids, scale=1.0):
     """scale * table[ids]: [*ids.shape, d] of the table's type.  A negative id gives a zero row, an id behind the table a row
     that is not a number."""
@@ -286,3 +300,12 @@ def check_step(users, items, user_vecs, item_vecs, b_i):
             raise TypeError("ranking_step: b_i must be a float32 ROCm tensor, which is updated in place")
         if b_i.shape != item_vecs.shape[:1]:
             raise ValueError("ranking_step: b_i must have an element for every item")
+    tables = [t for t in (user_vecs, item_vecs, b_i) if t is not None]
+    if any(s == 0 and n > 1 for t in tables for s, n in zip(t.stride(), t.shape)):
+        raise ValueError("ranking_step: a table that is updated in place must not hold an element twice")
+    if any(_share(a, b) and not (a is item_vecs and same_table(user_vecs, item_vecs)) for i, a in enumerate(tables) for b in tables[:i]):
+        raise ValueError("ranking_step: user_vecs, item_vecs and b_i must not share memory, unless user_vecs is item_vecs")
+
+
+def same_table(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()

@@ -669,6 +669,34 @@ def test_ranking_step_users_out_of_range():
     assert torch.equal(loss, want) and all(torch.equal(x, y) for x, y in zip(one, two))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_ranking_step_one_table(dtype):
+    """Users and items are rows of one table: one gradient, by which the step is clipped too."""
+    g = gen(39)
+    n, rows, d = 300, 400, 40
+    T, b = normal(g, rows, d, dtype=dtype), normal(g, rows)
+    u, i = ids_of(g, n, rows), ids_of(g, n, rows)
+    out, _ = loss_want(T.double()[u.long()], T, i, b, 0.3, torch.tensor(1.0 / n).cuda())
+    grad = out[3].index_add(0, u.long(), out[2])
+    norm = math.sqrt(float((grad ** 2).sum() + (out[4] ** 2).sum()))
+    want = T.double() - 0.5 * min(1.0, 0.02 / norm) * grad
+    loss, length = ra.ExplicitMF.ranking_step(u, i, T, T, b, lr=0.5, max_norm=0.02, scale=0.3)
+    # bf16: dx, dtable, their sum and the clipped gradient are rounded, half a step each of no more than the largest gradient row
+    rough = 1e-5 if dtype == F32 else 4 * half(BF16)
+    assert abs(float(length) / norm - 1) < rough
+    close(T, want, half(dtype) * want.abs() + 2 * U * want.abs() + 0.5 * 0.02 * rough)
+    close(loss, out[0], 1e-5 + torch.zeros_like(out[0]))
+
+
+def test_ranking_step_columns_of_one_buffer():
+    """Factors and biases as columns of one wider table: the same step as on tables of their own."""
+    u, i, P, Q, b = batch(40, users=700)
+    wide = torch.cat([P, Q, b[:, None]], 1)
+    loss, norm = ra.ExplicitMF.ranking_step(u, i, wide[:, :40], wide[:, 40:80], wide[:, 80], max_norm=0.05)
+    want, length = ra.ExplicitMF.ranking_step(u, i, P, Q, b, max_norm=0.05)
+    assert torch.equal(loss, want) and torch.equal(norm, length) and torch.equal(wide, torch.cat([P, Q, b[:, None]], 1))
+
+
 def test_ranking_step_tables_that_require_gradients():
     """All of them or one: the same step, and none of it recorded."""
     for which in ((0, 1, 2), (1,), (2,)):

@@ -81,6 +81,26 @@ def test_ranking_step_refusals(change, error):
         ra.ExplicitMF.ranking_step(**{**given, **change})
 
 
+def test_ranking_step_tables_of_their_own():
+    """One table inside the other, a table that holds an element twice: refused before anything is updated."""
+    both, users, items = torch.zeros(12, 8), _i(0, 1), _i(2, 3)
+    for user_vecs, item_vecs, b_i in ((both[:6], both[5:], None), (both, both[:11], None), (torch.zeros(1, 8).expand(9, 8), both, None),
+                                      (_x(9), torch.zeros(1, 8).expand(5, 8), None), (_x(9), both, torch.zeros(1).expand(12)),
+                                      (_x(9), both, both.view(-1)[:12]), (_x(9), both, both[:, 7]), (both[:, :5], both[:, 3:], None),
+                                      (both[:, 1:5], both[:, :4], None)):
+        with pytest.raises(ValueError, match="share memory|element twice"):
+            ra.ExplicitMF.ranking_step(users, items, user_vecs, item_vecs, b_i)
+
+
+def test_ranking_step_columns_of_one_table_are_apart():
+    if torch.cuda.is_available():
+        pytest.skip("GPU present")
+    wide, users, items = torch.zeros(12, 17), _i(0, 1), _i(2, 3)
+    for user_vecs, item_vecs, b_i in ((wide[:, :8], wide[:, 8:16], wide[:, 16]), (wide[:5, 9:], wide[:, 1:9], wide[:, 0]), (wide, wide, None)):
+        with pytest.raises(_abi.MfsgdError, match="no ROCm GPU"):               # nothing else is wrong with the call
+            ra.ExplicitMF.ranking_step(users, items, user_vecs, item_vecs, b_i)
+
+
 def test_no_gpu_no_answer():
     if torch.cuda.is_available():
         pytest.skip("GPU present")
