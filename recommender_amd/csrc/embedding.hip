@@ -392,8 +392,9 @@ __global__ __launch_bounds__(256) void k_row_sums(const T *__restrict__ grad, in
             T *dst = out + v * out_stride + c1;
             float was[V] = {};
             if (accumulate) load_vec<V>(dst, was);
+            const float f = any ? scale : 0.f;  // a row without tokens is zero whatever the scale is
 #pragma unroll
-            for (int q = 0; q < V; ++q) was[q] = fmaf(acc[q], scale, was[q]);
+            for (int q = 0; q < V; ++q) was[q] = fmaf(acc[q], f, was[q]);
             if (accumulate && c1 < c) {         // the columns of another lane: not a second time
 #pragma unroll
                 for (int q = 0; q < V; ++q) if (c1 + q >= c) store_f32(dst + q, was[q]);

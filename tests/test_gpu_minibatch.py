@@ -178,6 +178,22 @@ def test_embedding_grad_is_the_lookups():
     assert abs(left - right) <= 40 * U * size
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n, rows, d", [(40, 100, 8), (9000, 20000, 33)])
+def test_embedding_scale_that_is_no_number(dtype, scale, n, rows, d):
+    """Rows of no id and padding are zero whatever the scale is, and the others show it."""
+    ids = ids_of(gen(n), n, rows)
+    ids[3] = -1
+    ones = torch.ones(n, d, dtype=dtype, device="cuda")
+    named = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    named[ids[ids >= 0].long()] = True
+    grad = ra.embedding_grad(ones, ids, rows, scale=scale)
+    assert float(grad[~named].abs().sum()) == 0 and not bool(torch.isfinite(grad[named]).any())
+    out = ra.embedding(torch.ones(rows, d, dtype=dtype, device="cuda"), ids, scale=scale)
+    assert float(out[3].abs().sum()) == 0 and not bool(torch.isfinite(out[ids >= 0]).any())
+
+
 # ------------------------------------------------------------------ loss
 def loss_case(g, n, items, d, dtype, bias, spread=2.0):
     x = normal(g, n, d, dtype=dtype)
