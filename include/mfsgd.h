@@ -316,7 +316,12 @@ int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_
  * A logit of a row that is +inf (2.3e38 and more count as that) or not a number makes its loss, lse and gradients not a number;
  * so may any logit of an infinite float32 element.  A target whose logit is -inf otherwise has the loss +inf and probability 0.
  * 1e-20 <= scale <= 1e20, and bias / scale and bias * log2(e) have to be finite in float32 (or the bias -inf). */
-int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads);
+/* flags of the workspace call: for softmax_loss_grads; and, as a promise that needs less where the table is bfloat16 (no copy of
+ * it is kept for d of 32, 64, 128, 192 or 256): the table starts at a multiple of 16 bytes, its stride is a multiple of 8
+ * elements below 2^20. */
+#define MFSGD_WITH_GRADS 1
+#define MFSGD_TABLE_ALIGNED 2
+int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t flags);
 int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets,
                            const float *bias, int64_t n, int64_t n_items, int32_t d, float scale, int32_t dtype,
                            float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream);

@@ -815,16 +815,21 @@ int parts_of(int64_t n_sm, int64_t n_st, int64_t row_tiles, const PassShape &s, 
 
 struct LossPlan {
     int dp, planes, splits1, rt1, splits2, rt2;
-    bool conv;
+    bool conv, as_is;
     int64_t xp, wp, m1, s1, o1, init, q, g, s2, o2, bytes;
 };
 
-LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool grads)
+// Rows that start at multiples of 16 bytes, near enough for the tiles' 32-bit offsets
+bool rows_aligned(const void *p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && stride < (1 << 20); }
+
+// aligned: the table's rows are (rows_aligned)
+LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool grads, bool aligned)
 {
     LossPlan p = {};
     n = std::max<int64_t>(n, 1);
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
     p.planes = dtype == MFSGD_F32 ? 3 : 1;
+    p.as_is = p.planes == 1 && d == p.dp && aligned;           // a bf16 table whose rows are dp wide is the operand as it is
     const int mode1 = grads ? LOSS_SUMS : LOSS;
     auto shape = [&](int mode, bool conv) { return p.planes == 3 ? pass_shape<3>(p.dp, mode, conv) : pass_shape<1>(p.dp, mode, conv); };
     // Few row tiles convert the rows they stream on the way: a launch and a round trip to memory less (200 x 162541 x 64 fp32
@@ -841,7 +846,7 @@ LossPlan loss_plan(int64_t n, int64_t n_items, int32_t d, int32_t dtype, bool gr
     auto take = [&](int64_t bytes) { const int64_t o = at; at += align_up(bytes, 256); return o; };
     if (!p.conv) {
         if (grads) p.xp = take((int64_t)p.planes * n * p.dp * 2);
-        p.wp = take((int64_t)p.planes * n_items * p.dp * 2);       // not used where the table's rows are operands as they are
+        if (!p.as_is) p.wp = take((int64_t)p.planes * n_items * p.dp * 2);
     }
     p.m1 = take((int64_t)p.splits1 * n * 4);
     p.s1 = take((int64_t)p.splits1 * n * 4);
@@ -885,15 +890,13 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
               hipStream_t st)
 {
     constexpr int PL = sizeof(T) == 4 ? 3 : 1;
-    const LossPlan p = loss_plan(n, n_items, d, PL == 3 ? MFSGD_F32 : MFSGD_BF16, grads);
+    const LossPlan p = loss_plan(n, n_items, d, PL == 3 ? MFSGD_F32 : MFSGD_BF16, grads, rows_aligned(w, ws_));
     const Rows xr = {x, xs, (int32_t)n}, wr = {w, ws_, (int32_t)n_items};
-    // a bf16 table whose rows are dp wide and start at multiples of 16 bytes is the operand as it is
-    const bool as_is = PL == 1 && d == p.dp && ws_ % 8 == 0 && (uintptr_t)w % 16 == 0 && ws_ < (1 << 20);
     __bf16 *xp = (__bf16 *)(ws + p.xp), *wp = (__bf16 *)(ws + p.wp);
     if (!p.conv) {
         auto groups = [&](int64_t rows) { return (rows * (p.dp / 8) + 255) / 256; };
         const PlaneJob jx = {xr, targets, nullptr, xp}, jw = {wr, nullptr, bias, wp};
-        const int64_t gx = grads ? groups(n) : 0, gw = as_is ? 0 : groups(n_items);
+        const int64_t gx = grads ? groups(n) : 0, gw = p.as_is ? 0 : groups(n_items);
         if (gx + gw) hipLaunchKernelGGL((k_planes<T, PL>), grid_of(gx + gw), dim3(256), 0, st, jx, jw, gx, (int32_t)n_items, d, p.dp);
         MF_LAUNCH_CHECK();
     }
@@ -907,10 +910,10 @@ int loss_impl(const T *x, int64_t xs, const T *w, int64_t ws_, const int32_t *ta
     a.inv_scale = 1.f / scale;
     a.st = xr;
     a.sm = wr;
-    a.sm_planes = as_is ? (const __bf16 *)w : wp;
-    a.planes_stride = as_is ? ws_ : p.dp;
+    a.sm_planes = p.as_is ? (const __bf16 *)w : wp;
+    a.planes_stride = p.as_is ? ws_ : p.dp;
     a.plane = n_items * p.dp;
-    a.clear = as_is && bias;
+    a.clear = p.as_is && bias;
     a.splits = p.splits1; a.row_tiles = p.rt1;
     a.part_m = (float *)(ws + p.m1); a.part_s = (float *)(ws + p.s1); a.part_o = (float *)(ws + p.o1);
     if (const int rc = grads ? launch_stream_d<T, LOSS_SUMS>(p.dp, p.conv, a, st) : launch_stream_d<T, LOSS>(p.dp, p.conv, a, st)) return rc;
@@ -958,7 +961,7 @@ int check_loss(const char *who, const void *x, int64_t xs, const void *w, int64_
     MF_ARG(scale >= 1e-20f && scale <= 1e20f, "%s: scale must be from 1e-20 to 1e20", who);
     if (n == 0 && !grads) return MFSGD_OK;
     MF_ARG(w && (n == 0 || (x && targets && loss && lse)), "%s: null pointer", who);
-    const int64_t need = loss_plan(n, n_items, d, dtype, grads).bytes;
+    const int64_t need = loss_plan(n, n_items, d, dtype, grads, rows_aligned(w, ws_)).bytes;
     MF_ARG(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
     return MFSGD_OK;
 }
@@ -973,11 +976,11 @@ __global__ __launch_bounds__(256) void k_zero(T *__restrict__ p, int64_t n)
 
 extern "C" {
 
-int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t with_grads)
+int64_t mfsgd_softmax_loss_workspace(int64_t n, int64_t n_items, int32_t d, int32_t dtype, int32_t flags)
 {
     if (n < 0 || n > INT32_MAX / 4 || n_items < 1 || n_items > INT32_MAX / 4 || d < 1 || d > 256 || (dtype != MFSGD_F32 && dtype != MFSGD_BF16))
         return -1;
-    return loss_plan(n, n_items, d, dtype, with_grads != 0).bytes;
+    return loss_plan(n, n_items, d, dtype, flags & MFSGD_WITH_GRADS, flags & MFSGD_TABLE_ALIGNED).bytes;
 }
 
 int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, int64_t table_stride, const int32_t *targets, const float *bias,

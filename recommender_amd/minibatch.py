@@ -170,6 +170,11 @@ def _loss_args(x, table, targets, bias, scale):
     return x, xs, table, ts, targets, _vector(bias, table.shape[0], "bias")
 
 
+def _aligned(table, stride):
+    """MFSGD_TABLE_ALIGNED where it holds: the workspace then leaves out what only other tables need."""
+    return 2 if table.data_ptr() % 16 == 0 and stride % 8 == 0 and stride < 1 << 20 else 0
+
+
 def softmax_loss(x, table, targets, bias=None, scale=1.0):
     """Cross entropy of the softmax over all items: (loss [n], lse [n]) in float32, with the logits
     z = scale * x @ table.T + bias, lse = logsumexp(z), loss = lse - z[targets].  Rows of at most 256 elements.  A padding row
@@ -182,7 +187,7 @@ def softmax_loss(x, table, targets, bias=None, scale=1.0):
     n, d = x.shape
     with _On(x, table, targets, bias) as on:
         both = torch.empty((2, n), dtype=torch.float32, device=x.device)
-        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, table.shape[0], d, _DTYPES[x.dtype], 0))
+        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, table.shape[0], d, _DTYPES[x.dtype], _aligned(table, ts)))
         _abi.check(_abi.lib().mfsgd_hip_softmax_loss(
             x.data_ptr(), xs, table.data_ptr(), ts, targets.data_ptr(), None if bias is None else bias.data_ptr(), n,
             table.shape[0], d, scale, _DTYPES[x.dtype], both.data_ptr(), both.data_ptr() + 4 * n, ws.data_ptr(), ws.numel(),
@@ -204,7 +209,7 @@ def softmax_loss_grads(x, table, targets, bias=None, scale=1.0, weights=1.0):
         dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
         dtable = torch.empty((n_items, d), dtype=x.dtype, device=x.device)
         dbias = None if bias is None else torch.empty(n_items, dtype=torch.float32, device=x.device)
-        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, n_items, d, _DTYPES[x.dtype], 1))
+        ws = on.workspace(_abi.lib().mfsgd_softmax_loss_workspace(n, n_items, d, _DTYPES[x.dtype], 1 + _aligned(table, ts)))
         _abi.check(_abi.lib().mfsgd_hip_softmax_loss_grads(
             x.data_ptr(), xs, table.data_ptr(), ts, targets.data_ptr(), None if bias is None else bias.data_ptr(),
             None if each is None else each.data_ptr(), 1.0 if each is not None else float(weights), n, n_items, d, scale,

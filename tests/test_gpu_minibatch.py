@@ -542,6 +542,25 @@ def test_softmax_loss_strides():
     assert none[0].shape == (0,) and none[2].shape == (0, d) and float(none[3].abs().sum()) == 0
 
 
+def test_softmax_loss_workspace_holds_no_copy_of_the_table():
+    """A bf16 table of the operand's width is read where it is; one of another address is copied; the results are the same."""
+    n, items, d = 700, 40000, 128
+    x, w, t, b = loss_case(gen(13), n, items, d, BF16, True)
+    odd = torch.zeros(1 + items * d, dtype=BF16, device="cuda")[1:].view(items, d).copy_(w)
+
+    def call(table):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        loss = ra.softmax_loss(x, table, t, bias=b)
+        return loss, torch.cuda.max_memory_allocated() - before
+    (one, small), (two, large) = call(w), call(odd)
+    assert all(torch.equal(a, c) for a, c in zip(one, two))
+    assert small < w.numel() < large                     # half the table's bytes: the parts' sums are far fewer
+    got, want = ra.softmax_loss_grads(x, w, t, bias=b), ra.softmax_loss_grads(x, odd, t, bias=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
 def test_softmax_gradients_against_differences():
     """d/de of the 64-bit loss at x + e u, w + e v, b + e c, by central differences, is <dx, u> + <dw, v> + <db, c>."""
     g = gen(12)

@@ -155,6 +155,25 @@ def test_c_refusals_softmax_loss():
     assert "null" in _refused(lib.mfsgd_hip_softmax_loss(None, 8, p, 8, p, None, 4, 5, 8, 1.0, 0, p, p, p, need, None))
 
 
+def test_c_workspace_of_a_table_as_it_is():
+    """A bf16 table that is an operand as it is has no copy in the workspace; one that is not needs it, and the call says so."""
+    lib, p = _abi.lib(), 0x1000
+    size = lambda n, items, d, dtype, flags: lib.mfsgd_softmax_loss_workspace(n, items, d, dtype, flags)    # noqa: E731
+    for d, least in ((256, 624961 * 256 * 2), (32, 624961 * 32 * 2)):
+        for grads in (0, 1):
+            assert size(4096, 624961, d, 1, grads) - size(4096, 624961, d, 1, grads + 2) >= least
+    for n, items, d, dtype in ((4096, 9000, 100, 1), (4096, 9000, 64, 0), (3, 9000, 64, 1)):      # padded, split, or converted on the way
+        assert size(n, items, d, dtype, 1) == size(n, items, d, dtype, 3)
+    need = size(4096, 9000, 64, 1, 3)
+
+    def call(table=p, stride=64, nbytes=need):
+        return lib.mfsgd_hip_softmax_loss_grads(p, 64, table, stride, p, None, None, 1.0, 4096, 9000, 64, 1.0, 1, p, p, p, p, None, p, nbytes,
+                                                None)
+    assert "workspace" in _refused(call(nbytes=need - 1))
+    for kw in (dict(table=p + 2), dict(stride=65), dict(stride=1 << 20)):
+        assert "workspace" in _refused(call(**kw)), kw
+
+
 def test_c_refusals_clip():
     lib, p = _abi.lib(), 0x1000
     norm, ws = p + 0x100000, p + 0x200000
