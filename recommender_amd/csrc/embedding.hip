@@ -4,7 +4,7 @@
 //
 // The gradient sorts the batch's positions by id (stable: equal ids stay in the order of t), so that a table row's tokens
 // are one stretch of the sorted list; a row is then summed by one group of lanes in fp32, in the order of t, and written
-// once.  No floating-point atomics: the same inputs give the same bits.
+// once.  A popular row is cut where the sorted list is at multiples of 16 or 32, summed by many groups and joined.  No floating-point atomics: the same inputs give the same bits.
 //
 // 2 M tokens of 512 bytes into 480189 rows: 373 us, of which the sums take 270 (1.28 GB: 4.7 TB/s, a copy reaches 5.1) and the
 // sort and the rows' first places the rest.  131072 bf16 tokens of 256 bytes: 56 us, eight launches of 3 to 20 us that wait for

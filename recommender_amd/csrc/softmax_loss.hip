@@ -32,7 +32,7 @@
 // Types: bf16 rows are the operands as they are.  An fp32 row is split into three bf16 rows of 8 bits each (x = x0 + x1 + x2,
 // exact to 2^-24), and a product is the six products of order up to 2 - the three left out are below 2^-24 of it.  Six bf16
 // matrix instructions cost less than one fp32 instruction of the same shape (2.5 PFLOP/s against 157 TFLOP/s).  The
-// exponentials, too, are rounded to bf16 for the second product (bf16 rows: once, 2^-9 of a term, what the outputs themselves
+// exponentials, too, are rounded to bf16 for the second product (bf16 rows: once, by at most 2^-8 of a term, what the outputs themselves
 // are rounded by; in three parts it took 30 % more time.  fp32 rows: three parts, exact to 2^-24).  The sum of the
 // exponentials, lse, loss and 1 - p_t are of the unrounded ones.
 #include <algorithm>

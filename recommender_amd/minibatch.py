@@ -119,8 +119,8 @@ def embedding(table, ids, scale=1.0):
 
 
 def embedding_grad(grad, ids, n_rows, scale=1.0, out=None, accumulate=False):
-    """Gradient of `embedding` for its table: [n_rows, d], row v = scale * the sum of grad's rows whose id is v (in fp32, in the
-    order of ids), zero where no id is v.  `grad` is [*ids.shape, d].  With `out` the result is written there; with
+    """Gradient of `embedding` for its table: [n_rows, d], row v = scale * the sum of grad's rows whose id is v (in fp32; up to
+    16 of them in the order of ids, more in stretches that the whole batch's ids decide), zero where no id is v.  `grad` is [*ids.shape, d].  With `out` the result is written there; with
     `accumulate` it is added to `out` (one gradient of a table used twice; or, with scale = -learning rate, the update of the
     table itself), whose other rows stay untouched."""
     if not isinstance(grad, torch.Tensor) or grad.dim() < 1:
@@ -199,7 +199,8 @@ def softmax_loss(x, table, targets, bias=None, scale=1.0):
 def softmax_loss_grads(x, table, targets, bias=None, scale=1.0, weights=1.0):
     """(loss, lse, dx, dtable, dbias): `softmax_loss` and the gradients of sum(weights * loss).  `weights` is a number or a
     float32 tensor with an element for every row (1 / n: the mean over n rows).  dx and dtable have the type of x, summed in
-    fp32; dbias is float32, None without a bias."""
+    fp32 (of bfloat16 rows the probabilities, times a row's weight for dtable, are rounded to bfloat16 before they are multiplied;
+    not the target's share); dbias is float32, None without a bias."""
     x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
     n, d = x.shape
     n_items = table.shape[0]

@@ -155,6 +155,26 @@ def test_embedding_grad(dtype, n, rows, d, kind):
     assert torch.equal(base[(count == 0)[:, 0]], before[(count == 0)[:, 0]])
 
 
+@pytest.mark.parametrize("n, rows, d", [(900, 70, 8), (7000, 600, 33), (20000, 2000, 64)])
+def test_embedding_grad_order_of_few_tokens(n, rows, d):
+    """Rows of up to 16 tokens: the bits of the sum in the order of ids, whatever else is in the batch."""
+    g = gen(n)
+    ids = torch.arange(n, device="cuda", dtype=torch.int32) % rows
+    ids = ids[torch.randperm(n, device="cuda", generator=g)]
+    grad = normal(g, n, d)
+    by_id, place = torch.sort(ids.long(), stable=True)
+    first = torch.searchsorted(by_id, torch.arange(rows + 1, device="cuda"))
+    count = first[1:] - first[:-1]
+    assert int(count.max()) <= 16
+    want = torch.zeros(rows, d, device="cuda")
+    for k in range(16):                                           # every row's k-th token
+        here = torch.nonzero(k < count)[:, 0]
+        want[here] += grad[place[first[here] + k]]
+    assert torch.equal(ra.embedding_grad(grad, ids, rows), want)
+    more = torch.cat([ids, torch.full((100,), rows, dtype=torch.int32, device="cuda")])        # another row's tokens behind them
+    assert torch.equal(ra.embedding_grad(torch.cat([grad, grad[:100]]), more, rows + 1)[:rows], want)
+
+
 def test_embedding_grad_many_table_rows():
     """More lanes for the table's rows than a dimension of a grid has threads."""
     rows, d = (1 << 28) + 7, 33
