@@ -333,7 +333,7 @@ int mfsgd_hip_softmax_loss(const void *x, int64_t x_stride, const void *table, i
  * dx and dtable are without gaps, of `dtype`, rounded from fp32 sums.  Of bfloat16 rows each term of those sums but the target's
  * is a product of bfloat16 numbers: exp(z_rv - lse[r]), times weights[r] for dtable, is rounded to 8 bits (by at most 2^-8 of the
  * term) before it is multiplied, so that a row of dtable that no target names has a little more than its last rounding's error
- * (0.0019 instead of 0.0017 of it).  float32 rows keep 24 bits. */
+ * (0.0020 of it instead of 0.0017).  float32 rows keep 24 bits. */
 int mfsgd_hip_softmax_loss_grads(const void *x, int64_t x_stride, const void *table, int64_t table_stride,
                                  const int32_t *targets, const float *bias, const float *weights, float weight, int64_t n,
                                  int64_t n_items, int32_t d, float scale, int32_t dtype, float *loss, float *lse, void *dx,

@@ -528,8 +528,14 @@ GradPlan grad_plan(int64_t n, int64_t n_rows, int32_t d)
     // with 64), long ones write and read fewer parts (2 M tokens of fp32: 432, 405 and 402 us)
     p.hs = n <= RANK_MAX || n > 256 * 1024 ? 5 : 4;
     if (n > 1 << p.hs) p.parts = take(((n + (1 << p.hs) - 1) >> p.hs) * 2 * (int64_t)d * 4);
-    // A row's parts joined by one workgroup, or first 32 and 32 of them in a launch of their own (131072 tokens of 59047 rows 56
-    // us, 61 with that launch, all of them of one row 77 and 61; 262144 of one row 167 and 87)
+    // A row's parts joined by one workgroup, or first 32 and 32 of them in a launch of their own, which costs 2 to 6 us whatever the
+    // batch is and pays where one row has most of it; the host does not see how long the longest row is.  The bound is where a
+    // batch of one row alone would take more than twice an ordinary one's time without that launch.  Popular items of 59047, and
+    // all tokens of one row, d = 128, us without / with it:
+    //    65536 tokens  fp32 41 / 44 and  63 / 46    bf16 47 / 49 and  54 / 46
+    //   131072         fp32 49 / 54 and  98 / 61    bf16 56 / 62 and  76 / 61
+    //   196608         fp32 57 / 62 and 133 / 74    bf16 62 / 67 and  98 / 74
+    //   262144         fp32 66 / 71 and 167 / 88    bf16 67 / 72 and 124 / 90
     p.use_supers = n > 128 * 1024;
     if (p.use_supers) p.supers = take((n + (SUPER << p.hs) - 1) / (SUPER << p.hs) * 2 * (int64_t)d * 4);
     p.bytes = std::max<int64_t>(at, 256);
