@@ -317,7 +317,8 @@ int mfsgd_hip_embedding_grad(const void *grad, int64_t grad_stride, const int32_
  * no gradient, with every item out also the lse -inf.  A padding row's x is not looked at: loss and lse are 0.
  * A logit of a row that is +inf (2.3e38 and more count as that) or not a number makes its loss, lse and gradients not a number;
  * so may any logit of an infinite float32 element.  A target whose logit is -inf otherwise has the loss +inf and probability 0.
- * 1e-20 <= scale <= 1e20, and bias / scale and bias * log2(e) have to be finite in float32 (or the bias -inf). */
+ * 1e-20 <= scale <= 1e20, elements of x and table of at most 1e20 (a sum of exponentials of up to 2^61 times them is held in
+ * float32), and bias / scale and bias * log2(e) have to be finite in float32 (or the bias -inf). */
 /* flags of the workspace call: for softmax_loss_grads; and, as a promise that needs less where the table is bfloat16 (no copy of
  * it is kept for d of 32, 64, 128, 192 or 256): the table starts at a multiple of 16 bytes, its stride is a multiple of 8
  * elements below 2^20. */

@@ -182,7 +182,7 @@ def softmax_loss(x, table, targets, bias=None, scale=1.0):
     bias of -inf takes an item out of the catalogue, whatever its row holds; as a target it gives the loss +inf (and no
     gradient).  float32's lowest value does the same for an item whose row is finite; bias / scale has to stay in float32
     otherwise.  A logit that is +inf or not a number makes its row's loss and lse not a number, the target's logit as any other;
-    so may any logit of an infinite float32 element.  scale is from 1e-20 to 1e20."""
+    so may any logit of an infinite float32 element.  scale is from 1e-20 to 1e20; elements of x and table are of at most 1e20."""
     x, xs, table, ts, targets, bias = _loss_args(x, table, targets, bias, scale)
     n, d = x.shape
     with _On(x, table, targets, bias) as on:

@@ -459,15 +459,15 @@ def far_below_case(n, items, d, dtype, wide, high):
     return x, w, t, b, torch.rand(n, device="cuda", generator=g) + 0.5
 
 
-def far_below_holds(x, w, t, b, each):
+def far_below_holds(x, w, t, b, each, scale=1.0):
     n, (items, d) = x.shape[0], w.shape
-    out, mass = loss_want(x, w, t, b, 1.0, each)
+    out, mass = loss_want(x, w, t, b, torch.tensor(scale, dtype=F32).double().item(), each)
     assert float(out[0].min()) > 80
     tol = loss_tolerances(out, mass, n, items, d, x.dtype)
-    loss, lse = ra.softmax_loss(x, w, t, bias=b)
+    loss, lse = ra.softmax_loss(x, w, t, bias=b, scale=scale)
     close(loss, out[0], tol[0])
     close(lse, out[1], tol[1])
-    got = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+    got = ra.softmax_loss_grads(x, w, t, bias=b, scale=scale, weights=each)
     for k in range(5):
         close(got[k], out[k], tol[k])
 
@@ -478,6 +478,15 @@ def test_softmax_loss_target_far_below(dtype, n, d, wide):
     """The first items set a low reference, the sum stands 2^58 above it and the target 2^63 below: fp32 has to hold what the
     join makes of them, times the items' elements."""
     far_below_holds(*far_below_case(n, 64, d, dtype, wide, [50]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, items, d", [(5, 64, 8), (140, 700, 40), (600, 300, 128)])
+def test_softmax_loss_largest_elements(dtype, n, items, d):
+    """Elements up to 1e20, the smallest scale, and sums 2^58 above their references: all within fp32."""
+    x, w, t, b, each = far_below_case(n, items, d, dtype, 3e19, [50])
+    x = normal(gen(d), n, d, dtype=dtype, std=1e-2)
+    far_below_holds(x, w.clamp(-9.9e19, 9.9e19), t, b, each, scale=1e-20)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -789,6 +798,40 @@ def test_captured_step_replays():
         torch.cuda.synchronize()
         assert torch.equal(loss, loss2) and torch.equal(norm, norm2)
         assert all(torch.equal(a, c) for a, c in zip((P, Q, b), mine))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_wide_and_large_calls(dtype):
+    """The widest rows (more than 64 KB of LDS a workgroup) and a batch whose popular rows are joined in two steps, in one graph,
+    replayed with other inputs and eager calls in between."""
+    def inputs(seed):
+        g = gen(seed)
+        x, w, t, b = loss_case(g, 600, 3000, 256, dtype, True)
+        ids = torch.where(torch.rand(300000, device="cuda", generator=g) < 0.5, 7, ids_of(g, 300000, 3000)).int()
+        return [x, w, t, b, normal(g, 300000, 40, dtype=dtype), ids]
+
+    def step(x, w, t, b, grad, ids):
+        loss, lse, dx, dw, db = ra.softmax_loss_grads(x, w, t, bias=b, weights=1.0 / 600)
+        de = ra.embedding_grad(grad, ids, 3000)
+        norm = ra.clip_grads([dx, dw, db, de], 0.5)
+        return [loss, lse, dx, dw, db, de, norm, ra.embedding(de, ids), *ra.softmax_loss(x, w, t, bias=b)]
+    held = inputs(50)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    for seed in (51, 52, 53, 54):
+        new = inputs(seed)
+        for a, b in zip(held, new):
+            a.copy_(b)
+        graph.replay()
+        want = step(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
 def test_two_streams_at_once():
