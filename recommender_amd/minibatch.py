@@ -120,9 +120,9 @@ def embedding(table, ids, scale=1.0):
 
 def embedding_grad(grad, ids, n_rows, scale=1.0, out=None, accumulate=False):
     """Gradient of `embedding` for its table: [n_rows, d], row v = scale * the sum of grad's rows whose id is v (in fp32; up to
-    16 of them in the order of ids, more in stretches that the whole batch's ids decide), zero where no id is v.  `grad` is [*ids.shape, d].  With `out` the result is written there; with
-    `accumulate` it is added to `out` (one gradient of a table used twice; or, with scale = -learning rate, the update of the
-    table itself), whose other rows stay untouched."""
+    16 of them in the order of ids, more in stretches that the whole batch's ids decide), zero where no id is v.  `grad` is
+    [*ids.shape, d].  With `out` the result is written there; with `accumulate` it is added to `out` (one gradient of a table
+    used twice; or, with scale = -learning rate, the update of the table itself), whose other rows stay untouched."""
     if not isinstance(grad, torch.Tensor) or grad.dim() < 1:
         raise ValueError("grad must be a tensor")
     ids = _ids(ids, "ids")
@@ -307,10 +307,20 @@ def check_step(users, items, user_vecs, item_vecs, b_i):
         if b_i.shape != item_vecs.shape[:1]:
             raise ValueError("ranking_step: b_i must have an element for every item")
     tables = [t for t in (user_vecs, item_vecs, b_i) if t is not None]
-    if any(s == 0 and n > 1 for t in tables for s, n in zip(t.stride(), t.shape)):
+    if not all(_once(t) for t in tables):
         raise ValueError("ranking_step: a table that is updated in place must not hold an element twice")
     if any(_share(a, b) and not (a is item_vecs and same_table(user_vecs, item_vecs)) for i, a in enumerate(tables) for b in tables[:i]):
         raise ValueError("ranking_step: user_vecs, item_vecs and b_i must not share memory, unless user_vecs is item_vecs")
+
+
+def _once(t):
+    """Whether every element has a place of its own: each dimension steps over all that the ones with smaller steps reach."""
+    reach = 0
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s <= reach:
+            return False
+        reach += s * (n - 1)
+    return True
 
 
 def same_table(a, b):

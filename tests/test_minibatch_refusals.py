@@ -87,7 +87,7 @@ def test_ranking_step_tables_of_their_own():
     for user_vecs, item_vecs, b_i in ((both[:6], both[5:], None), (both, both[:11], None), (torch.zeros(1, 8).expand(9, 8), both, None),
                                       (_x(9), torch.zeros(1, 8).expand(5, 8), None), (_x(9), both, torch.zeros(1).expand(12)),
                                       (_x(9), both, both.view(-1)[:12]), (_x(9), both, both[:, 7]), (both[:, :5], both[:, 3:], None),
-                                      (both[:, 1:5], both[:, :4], None)):
+                                      (both[:, 1:5], both[:, :4], None), (_x(9), torch.zeros(20).as_strided((5, 8), (3, 1)), None)):
         with pytest.raises(ValueError, match="share memory|element twice"):
             ra.ExplicitMF.ranking_step(users, items, user_vecs, item_vecs, b_i)
 
