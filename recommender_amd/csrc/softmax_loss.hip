@@ -708,7 +708,7 @@ __global__ __launch_bounds__(64 * W) void k_join_rows(const JoinArgs a, const T 
     const float g = a.weights ? a.weights[r] : 1.f;
     if (lane == 0 && wave == 0) {
         a.row_init[r] = none ? -INFINITY : -((log_all + ref * LN2) / a.scale);
-        a.row_q[r] = q * g;
+        a.row_q[r] = none ? 0.f : q * g;
         if (a.row_g) a.row_g[r] = none ? 0.f : g;
     }
     // four columns a lane, the parts dealt to 64 / lanes groups of lanes

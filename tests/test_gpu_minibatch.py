@@ -337,6 +337,24 @@ def test_softmax_loss_masks(dtype, n, d):
     assert float(dx.abs().sum()) == 0 and float(dw.abs().sum()) == 0 and float(db.abs().sum()) == 0
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [40, 700])
+@pytest.mark.parametrize("weight", [math.inf, math.nan])
+def test_softmax_loss_no_gradient_whatever_the_weight(dtype, n, weight):
+    """Padding and a row whose target is out of the catalogue have no gradient, and their weights are not looked at."""
+    g = gen(83)
+    x, w, t, b = loss_case(g, n, 300, 64, dtype, True)
+    b[20] = -math.inf
+    t[t == 20] = 21
+    t[0], t[1] = 20, -1
+    each = torch.rand(n, device="cuda", generator=g)
+    each[:2] = 0.0
+    want = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+    each[:2] = weight
+    got = ra.softmax_loss_grads(x, w, t, bias=b, weights=each)
+    assert all(bool(torch.isfinite(v).all()) for v in got[2:]) and all(torch.equal(a, c) for a, c in zip(got, want))
+
+
 def test_softmax_loss_first_items_masked():
     """No item of the catalogue among the first ones: the sums' reference is set late, and far from the masked zeros."""
     n, items, d = 40, 400, 32
