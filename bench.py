@@ -31,7 +31,7 @@ def bytes_per_update(k, implicit):
 
 def kernel_source_hash():
     """Identifies the build a PMC record in profiles/traffic.json belongs to: sha256 over the sources of the epoch kernel
-    (csrc/epoch.hip, csrc/common.h - the GPU box has no .git) and the compiler flags that the Makefile gives them.
+    (csrc/epoch.hip, csrc/common.h - not every copy of the tree has a .git) and the compiler flags that the Makefile gives them.
     profiles/collect_traffic.py stores the same hash with every record it writes."""
     import hashlib
     import re
